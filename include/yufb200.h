@@ -178,6 +178,82 @@ yuf_status_t yuf_rosa_backward(const float* cand_saved, const float* write_saved
                                float* d_memory_out, float* workspace, int B, int T, int R,
                                void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Gated recurrence and dropout: operators for recurrent blocks beside WKV-7 and
+ * ROSA.  No reference counterpart.  Unlike the rest of this header their
+ * per-token tensors may be bf16 or fp16, and rows may be strided.
+ * ------------------------------------------------------------------------ */
+enum { YUF_DTYPE_F32 = 0, YUF_DTYPE_BF16 = 1, YUF_DTYPE_F16 = 2 };
+
+/* Elementwise gated recurrence (per channel of [B, T, D], fp32 inside):
+ *   a_t = lower + (1 - lower) sigmoid(forget_t)
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t
+ *   y_t = h_t sigmoid(gate_t)            (y_t = h_t when gate is NULL)
+ *   x, forget, gate : [B, T, D] of `dtype`, unit stride along D; strides [6] (host)
+ *                     = batch and token stride of each in elements, NULL = contiguous
+ *   lower           : [D] fp32 retention floor in [0, 1), NULL = 0
+ *   h0              : [B, D] fp32 initial state ([n_seqs, D] when packed), NULL = 0
+ *   cu_seqlens      : NULL, or device [n_seqs + 1], non-decreasing: B must be 1 and
+ *                     rows cu[s] .. cu[s+1] - 1 are sequence s, each with its own
+ *                     state; a sequence may be empty.  Rows in no sequence are not
+ *                     read and get y = 0.  The contents are not checked (wrong ones
+ *                     give wrong values, never an access out of bounds).
+ *   y               : [B, T, D] of `dtype`, contiguous
+ *   h_last          : [B, D] ([n_seqs, D]) fp32 final state, or NULL.  An empty
+ *                     sequence's is its h0.  Must not overlap h0.
+ *   checkpoints     : [B, ceil(T / block), D] fp32 or NULL: the state before every
+ *                     block of yuf_gated_scan_block(dtype) tokens, for the backward.
+ * Outputs must not overlap inputs.  Any T <= 2^30, any D. */
+yuf_status_t yuf_gated_scan_forward(const void* x, const void* forget, const void* gate,
+                                    const int64_t* strides, const float* lower, const float* h0,
+                                    const int32_t* cu_seqlens, int n_seqs, void* y, float* h_last,
+                                    float* checkpoints, int dtype, int B, int T, int D,
+                                    void* stream);
+/* Tokens between two checkpoints for an element type (0: unknown type). */
+int yuf_gated_scan_block(int dtype);
+/* Rows of the backward's `partial` buffer. */
+int64_t yuf_gated_scan_partial_rows(int B, int T, int D, int dtype);
+/* Gradients of the forward, given dy = dL/dy [B, T, D] of `dtype` (strides [8]:
+ * x, forget, gate, dy) and dh_last = dL/dh_last fp32 (NULL = zeros), from the same
+ * inputs and the checkpoints it wrote:
+ *   dx, dforget, dgate : [B, T, D] of `dtype`, contiguous; zero in rows of no
+ *                        sequence.  dgate is NULL exactly when gate is.
+ *   dlower             : [D] fp32 or NULL; needs `partial`, a caller's buffer of
+ *                        yuf_gated_scan_partial_rows x D floats (its contents before
+ *                        the call do not matter)
+ *   dh0                : [B, D] ([n_seqs, D]) fp32 or NULL
+ * Every sum has a fixed order: the same call gives the same bits. */
+yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const void* gate,
+                                     const void* dy, const int64_t* strides, const float* lower,
+                                     const float* h0, const int32_t* cu_seqlens, int n_seqs,
+                                     const float* checkpoints, const float* dh_last, void* dx,
+                                     void* dforget, void* dgate, float* dlower, float* dh0,
+                                     float* partial, int dtype, int B, int T, int D, void* stream);
+/* One token of B sequences: x, forget, gate (or NULL) [B, D] with row strides
+ * strides [3] (NULL = contiguous), y [B, D] contiguous; state [B, D] fp32 with row
+ * stride state_stride (>= D) is updated in place, e.g. a slot range of a pool. */
+yuf_status_t yuf_gated_scan_step(const void* x, const void* forget, const void* gate,
+                                 const int64_t* strides, const float* lower, float* state,
+                                 int64_t state_stride, void* y, int dtype, int B, int D,
+                                 void* stream);
+
+/* Dropout with a mask that is never stored, and an optional residual add:
+ *   out_i = residual_i + (w_i >= floor(p 2^32) ? x_i / (1 - p) : 0)
+ * with w_i = word i % 4 of Philox4x32-10(key = seed, counter = (i / 4, step)) and i
+ * the element's row-major index in [rows, cols].  p = 1 drops everything.  The
+ * backward is the same call on dy without a residual: same seed, step, rows and
+ * cols draw the same words.  x [rows, cols] has row stride x_stride; residual (or
+ * NULL) has out's type and row stride residual_stride; out is contiguous and may be
+ * the residual's own buffer when that is contiguous too (or x's, same type).
+ * Types (x, out): equal ones; bf16 or fp16 x with fp32 out (an fp32 residual
+ * stream); fp32 x with bf16 or fp16 out and no residual (that call's gradient).
+ * step_device (device, 8 bytes), when not NULL, is read instead of `step`, so a
+ * captured graph draws new masks as the caller advances it. */
+yuf_status_t yuf_dropout(const void* x, int64_t x_stride, int x_dtype, const void* residual,
+                         int64_t residual_stride, void* out, int out_dtype, int64_t rows,
+                         int64_t cols, double p, uint64_t seed, uint64_t step,
+                         const uint64_t* step_device, void* stream);
+
 /* Projection GEMM of the engine (bf16 operands, fp32 accumulation, tcgen05
  * tensor cores), the nn.Linear products of yufmusicgen/model.py:107-112,
  * 195-197, 297-311, 376-377, 421 for a host that drives the block itself:

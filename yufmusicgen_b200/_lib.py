@@ -27,6 +27,11 @@ SIGNATURES = {
     "yuf_rosa_forward_compat": [P] * 14 + [I] * 3 + [P],
     "yuf_wkv7_backward": [P] * 15 + [I] * 4 + [P],
     "yuf_rosa_backward": [P] * 16 + [I] * 3 + [P],
+    "yuf_gated_scan_forward": [P, P, P, P, P, P, P, I, P, P, P, I, I, I, I, P],
+    "yuf_gated_scan_backward": [P] * 8 + [I] + [P] * 8 + [I] * 4 + [P],
+    "yuf_gated_scan_step": [P] * 6 + [ctypes.c_int64, P, I, I, I, P],
+    "yuf_dropout": [P, ctypes.c_int64, I, P, ctypes.c_int64, P, I, ctypes.c_int64, ctypes.c_int64, ctypes.c_double,
+                    ctypes.c_uint64, ctypes.c_uint64, P, P],
     "yuf_model_create": [P, I, I, I, P, P, P, P],
     "yuf_model_create_from_yuf": [ctypes.c_char_p, I, I, P],
     "yuf_model_destroy": [P],
@@ -112,6 +117,9 @@ def load():
         lib.yuf_abi_version.restype = I
         lib.yuf_wait_timeouts.restype = ctypes.c_uint
         lib.yuf_wait_timeouts.argtypes = []
+        lib.yuf_gated_scan_block.argtypes = [I]
+        lib.yuf_gated_scan_partial_rows.restype = ctypes.c_int64
+        lib.yuf_gated_scan_partial_rows.argtypes = [I] * 4
         for name, args in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.argtypes = args

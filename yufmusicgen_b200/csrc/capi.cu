@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <mutex>
 
+#include "gated_scan.cuh"
 #include "model_kernels.cuh"
 
 namespace yuf {
@@ -338,6 +339,146 @@ yuf_status_t yuf_rosa_backward(const float* cand_saved, const float* write_saved
   return rosa_backward_dispatch(cand_saved, write_saved, decay_saved, mem_saved, direction, d_read,
                                 d_cand, d_write, d_read_raw, d_decay, d_direction_partial,
                                 d_memory_out, B, T, R, static_cast<cudaStream_t>(stream));
+}
+
+// ---- gated recurrence and dropout -----------------------------------------
+
+static bool known_dtype(int d) { return d == YUF_DTYPE_F32 || d == YUF_DTYPE_BF16 || d == YUF_DTYPE_F16; }
+static size_t dtype_size(int d) { return d == YUF_DTYPE_F32 ? 4 : 2; }
+
+// Shared checks and fields of the two gated-scan calls; `in` = x, forget, gate, dy.
+static yuf_status_t gated_scan_args(const char* who, const void* const in[4], const int64_t* strides, int n_in,
+                                    const float* lower, const float* h0, const int32_t* cu_seqlens, int n_seqs,
+                                    int dtype, int B, int T, int D, yuf::GatedScanArgs& a) {
+  REQUIRE(known_dtype(dtype), "%s: unknown element type %d", who, dtype);
+  REQUIRE(B >= 0 && T >= 0 && D >= 1, "%s: bad size (B=%d T=%d D=%d)", who, B, T, D);
+  REQUIRE(T <= (1 << 30), "%s: T=%d is above 2^30", who, T);
+  REQUIRE((long long)B * ((D + 31) / 32) <= (1LL << 26), "%s: B=%d x D=%d is too large", who, B, D);
+  REQUIRE(!cu_seqlens || (B == 1 && n_seqs >= 0), "%s: packed sequences need B = 1 and n_seqs >= 0 (B=%d n_seqs=%d)",
+          who, B, n_seqs);
+  REQUIRE(aligned(cu_seqlens, 4) && aligned(lower, 4) && aligned(h0, 4), "%s: a buffer is not 4-byte aligned", who);
+  long long st[8];
+  for (int k = 0; k < 4; ++k) {
+    st[2 * k] = strides && k < n_in ? strides[2 * k] : (long long)T * D;
+    st[2 * k + 1] = strides && k < n_in ? strides[2 * k + 1] : D;
+    REQUIRE(st[2 * k] >= 0 && st[2 * k + 1] >= 0, "%s: negative stride", who);
+    REQUIRE(aligned(in[k], dtype_size(dtype)), "%s: a tensor is not aligned to its elements", who);
+  }
+  const bool rows = (long long)B * T > 0;
+  REQUIRE(!rows || (in[0] && in[1]), "%s: x and forget are required", who);
+  a = yuf::GatedScanArgs{};
+  a.x = in[0]; a.f = in[1]; a.g = in[2]; a.dy = in[3];
+  a.xb = st[0]; a.xt = st[1]; a.fb = st[2]; a.ft = st[3];
+  // tensors that are not there do not hold back the two-channel form
+  if (in[2]) { a.gb = st[4]; a.gt = st[5]; }
+  if (in[3]) { a.yb = st[6]; a.yt = st[7]; }
+  a.lower = lower; a.h0 = h0; a.cu = cu_seqlens; a.n_seqs = cu_seqlens ? n_seqs : 0;
+  a.B = B; a.T = T; a.D = D; a.dtype = dtype;
+  return YUF_OK;
+}
+
+int yuf_gated_scan_block(int dtype) { return known_dtype(dtype) ? yuf::gated_scan_block(dtype) : 0; }
+
+int64_t yuf_gated_scan_partial_rows(int B, int T, int D, int dtype) {
+  if (!known_dtype(dtype) || B < 0 || T < 0 || D < 1) return 0;
+  return yuf::gated_scan_partial_rows(B, T, D);
+}
+
+yuf_status_t yuf_gated_scan_forward(const void* x, const void* forget, const void* gate, const int64_t* strides,
+                                    const float* lower, const float* h0, const int32_t* cu_seqlens, int n_seqs,
+                                    void* y, float* h_last, float* checkpoints, int dtype, int B, int T, int D,
+                                    void* stream) {
+  g_err[0] = 0;
+  yuf::GatedScanArgs a;
+  const void* in[4] = {x, forget, gate, nullptr};
+  yuf_status_t st =
+      gated_scan_args("gated scan", in, strides, 3, lower, h0, cu_seqlens, n_seqs, dtype, B, T, D, a);
+  if (st != YUF_OK) return st;
+  REQUIRE((long long)B * T == 0 || y, "gated scan: y is required");
+  REQUIRE(aligned(y, dtype_size(dtype)) && aligned(h_last, 4) && aligned(checkpoints, 4),
+          "gated scan: an output is not aligned to its elements");
+  if (B == 0) return YUF_OK;
+  a.y = y; a.h_last = h_last; a.ckpt = checkpoints;
+  return yuf::gated_scan_forward(a, static_cast<cudaStream_t>(stream));
+}
+
+yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const void* gate, const void* dy,
+                                     const int64_t* strides, const float* lower, const float* h0,
+                                     const int32_t* cu_seqlens, int n_seqs, const float* checkpoints,
+                                     const float* dh_last, void* dx, void* dforget, void* dgate, float* dlower,
+                                     float* dh0, float* partial, int dtype, int B, int T, int D, void* stream) {
+  g_err[0] = 0;
+  yuf::GatedScanArgs a;
+  const void* in[4] = {x, forget, gate, dy};
+  yuf_status_t st =
+      gated_scan_args("gated scan backward", in, strides, 4, lower, h0, cu_seqlens, n_seqs, dtype, B, T, D, a);
+  if (st != YUF_OK) return st;
+  REQUIRE((long long)B * T == 0 || (dy && dx && dforget && checkpoints),
+          "gated scan backward: dy, dx, dforget and checkpoints are required");
+  REQUIRE((long long)B * T == 0 || !gate || dgate, "gated scan backward: dgate is required with a gate");
+  REQUIRE(B == 0 || !dlower || partial, "gated scan backward: dlower needs the partial buffer");
+  const size_t e = dtype_size(dtype);
+  REQUIRE(aligned(dx, e) && aligned(dforget, e) && aligned(dgate, e) && aligned(dlower, 4) && aligned(dh0, 4) &&
+              aligned(partial, 4) && aligned(checkpoints, 4) && aligned(dh_last, 4),
+          "gated scan backward: a buffer is not aligned to its elements");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (B == 0) {
+    if (dlower && cudaMemsetAsync(dlower, 0, (size_t)D * sizeof(float), s) != cudaSuccess)
+      return check_launch("gated scan backward: memset");
+    return YUF_OK;
+  }
+  a.ckpt = const_cast<float*>(checkpoints); a.dh_last = dh_last;
+  a.dx = dx; a.df = dforget; a.dg = gate ? dgate : nullptr;
+  a.dlower = dlower; a.dh0 = dh0; a.partial = dlower ? partial : nullptr;
+  return yuf::gated_scan_backward(a, s);
+}
+
+yuf_status_t yuf_gated_scan_step(const void* x, const void* forget, const void* gate, const int64_t* strides,
+                                 const float* lower, float* state, int64_t state_stride, void* y, int dtype, int B,
+                                 int D, void* stream) {
+  g_err[0] = 0;
+  REQUIRE(known_dtype(dtype), "gated scan step: unknown element type %d", dtype);
+  REQUIRE(B >= 0 && D >= 1, "gated scan step: bad size (B=%d D=%d)", B, D);
+  REQUIRE((long long)B * D <= (1LL << 38), "gated scan step: B=%d x D=%d is too large", B, D);
+  if (B == 0) return YUF_OK;
+  REQUIRE(x && forget && state && y, "gated scan step: x, forget, state and y are required");
+  const size_t e = dtype_size(dtype);
+  REQUIRE(aligned(x, e) && aligned(forget, e) && aligned(gate, e) && aligned(y, e) && aligned(state, 4) &&
+              aligned(lower, 4),
+          "gated scan step: a buffer is not aligned to its elements");
+  const long long xs = strides ? strides[0] : D, fs = strides ? strides[1] : D, gs = strides && gate ? strides[2] : D;
+  REQUIRE(xs >= 0 && fs >= 0 && gs >= 0, "gated scan step: negative stride");
+  REQUIRE(B == 1 || state_stride >= D, "gated scan step: state rows overlap (stride %lld, D=%d)",
+          (long long)state_stride, D);
+  return yuf::gated_scan_step(x, forget, gate, xs, fs, gate ? gs : 0, lower, state, B == 1 ? 0 : state_stride, y,
+                              dtype, B, D, static_cast<cudaStream_t>(stream));
+}
+
+yuf_status_t yuf_dropout(const void* x, int64_t x_stride, int x_dtype, const void* residual, int64_t residual_stride,
+                         void* out, int out_dtype, int64_t rows, int64_t cols, double p, uint64_t seed, uint64_t step,
+                         const uint64_t* step_device, void* stream) {
+  g_err[0] = 0;
+  REQUIRE(known_dtype(x_dtype) && known_dtype(out_dtype), "dropout: unknown element type (%d, %d)", x_dtype, out_dtype);
+  REQUIRE(p >= 0.0 && p <= 1.0, "dropout: p=%g is outside [0, 1]", p);
+  REQUIRE(rows >= 0 && cols >= 0, "dropout: negative size (rows=%lld cols=%lld)", (long long)rows, (long long)cols);
+  REQUIRE(cols == 0 || rows <= (1LL << 40) / cols, "dropout: tensor too large");
+  if (rows == 0 || cols == 0) return YUF_OK;
+  REQUIRE(x && out, "dropout: x and out are required");
+  REQUIRE(x_stride >= 0 && residual_stride >= 0, "dropout: negative stride");
+  REQUIRE(aligned(x, dtype_size(x_dtype)) && aligned(residual, dtype_size(out_dtype)) &&
+              aligned(out, dtype_size(out_dtype)) && aligned(step_device, 8),
+          "dropout: a buffer is not aligned to its elements");
+  yuf::DropoutArgs a{};
+  a.x = x; a.res = residual; a.out = out;
+  a.xs = x_stride; a.rs = residual_stride;
+  a.rows = rows; a.cols = cols;
+  a.x_dtype = x_dtype; a.out_dtype = out_dtype;
+  const uint64_t limit = static_cast<uint64_t>(p * 4294967296.0);  // exact: a power of two
+  a.any = limit > 0;
+  a.last_dropped = static_cast<uint32_t>(limit - 1);
+  a.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
+  a.seed = seed; a.step = step; a.step_ptr = step_device;
+  return yuf::dropout_forward(a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

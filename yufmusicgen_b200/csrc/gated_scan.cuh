@@ -1,0 +1,50 @@
+// Arguments of the gated recurrence's kernels (gated_scan.cu), filled by the
+// C ABI (ops_capi.cu).
+#pragma once
+#include "common.cuh"
+
+namespace yuf {
+
+struct GatedScanArgs {
+  const void *x, *f, *g, *dy;                        // inputs; g and dy may be NULL
+  long long xb, xt, fb, ft, gb, gt, yb, yt;          // batch and token strides of x, f, g, dy (elements)
+  const float *lower, *h0;                           // [D], [rows, D]; NULL = zeros
+  const int* cu;                                     // [n_seqs + 1] or NULL
+  int n_seqs;
+  int B, T, D;
+  int dtype;
+  // forward
+  void* y;
+  float *h_last, *ckpt;                              // either may be NULL (ckpt is an input of the backward)
+  // backward
+  const float* dh_last;                              // NULL = zeros
+  void *dx, *df, *dg;
+  float *dlower, *dh0, *partial;
+};
+
+// tokens between two saved states, by element type
+constexpr int gated_scan_block(int dtype) { return dtype == YUF_DTYPE_F32 ? 8 : 16; }
+// rows of `partial` the backward writes
+long long gated_scan_partial_rows(int B, int T, int D);
+
+yuf_status_t gated_scan_forward(const GatedScanArgs& a, cudaStream_t st);
+yuf_status_t gated_scan_backward(const GatedScanArgs& a, cudaStream_t st);
+yuf_status_t gated_scan_step(const void* x, const void* f, const void* g, long long xs, long long fs,
+                             long long gs, const float* lower, float* state, long long ss, void* y, int dtype,
+                             int B, int D, cudaStream_t st);
+
+struct DropoutArgs {
+  const void *x, *res;        // res may be NULL
+  void* out;
+  long long xs, rs;           // row strides of x and res (out is contiguous)
+  long long rows, cols;
+  int x_dtype, out_dtype;     // res has out's type
+  uint32_t last_dropped;      // an element is dropped when any && its word <= last_dropped
+  bool any;
+  float scale;
+  uint64_t seed, step;
+  const uint64_t* step_ptr;   // device; overrides step when not NULL
+};
+yuf_status_t dropout_forward(const DropoutArgs& a, cudaStream_t st);
+
+}  // namespace yuf

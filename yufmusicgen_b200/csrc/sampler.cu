@@ -21,27 +21,9 @@
 #include <cfloat>
 
 #include "common.cuh"
+#include "philox.cuh"
 
 namespace yuf {
-
-struct U4 {
-  uint32_t x, y, z, w;
-};
-
-// Philox4x32-10 as published (round multipliers and Weyl key increments).
-YUF_DEVICE U4 philox4x32_10(U4 c, uint32_t k0, uint32_t k1) {
-  constexpr uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u;
-  constexpr uint32_t W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(M0, c.x), lo0 = M0 * c.x;
-    const uint32_t hi1 = __umulhi(M1, c.z), lo1 = M1 * c.z;
-    c = U4{hi1 ^ c.y ^ k0, lo1, hi0 ^ c.w ^ k1, lo0};
-    k0 += W0;
-    k1 += W1;
-  }
-  return c;
-}
 
 YUF_DEVICE float philox_uniform(uint64_t seed, uint64_t step, uint32_t seq) {
   const U4 out = philox4x32_10(U4{(uint32_t)step, (uint32_t)(step >> 32), seq, 0u}, (uint32_t)seed,
