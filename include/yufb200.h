@@ -203,32 +203,34 @@ enum { YUF_DTYPE_F32 = 0, YUF_DTYPE_BF16 = 1, YUF_DTYPE_F16 = 2 };
  *                     sequence's is its h0.  Must not overlap h0.
  *   checkpoints     : [B, ceil(T / block), D] fp32 or NULL: the state before every
  *                     block of yuf_gated_scan_block(dtype) tokens, for the backward.
+ *   workspace       : yuf_gated_scan_workspace_bytes bytes of device memory, 16-byte
+ *                     aligned (NULL where that is 0); its contents before the call do
+ *                     not matter, and calls that may run at once need one each
  * Outputs must not overlap inputs.  Any T <= 2^30, any D. */
 yuf_status_t yuf_gated_scan_forward(const void* x, const void* forget, const void* gate,
                                     const int64_t* strides, const float* lower, const float* h0,
                                     const int32_t* cu_seqlens, int n_seqs, void* y, float* h_last,
-                                    float* checkpoints, int dtype, int B, int T, int D,
-                                    void* stream);
+                                    float* checkpoints, void* workspace, int dtype, int B, int T,
+                                    int D, void* stream);
 /* Tokens between two checkpoints for an element type (0: unknown type). */
 int yuf_gated_scan_block(int dtype);
-/* Rows of the backward's `partial` buffer. */
-int64_t yuf_gated_scan_partial_rows(int B, int T, int D, int dtype);
+/* Bytes of the workspace that a call of this size needs (backward = 0 or 1). */
+size_t yuf_gated_scan_workspace_bytes(int B, int T, int D, int dtype, int backward);
 /* Gradients of the forward, given dy = dL/dy [B, T, D] of `dtype` (strides [8]:
  * x, forget, gate, dy) and dh_last = dL/dh_last fp32 (NULL = zeros), from the same
  * inputs and the checkpoints it wrote:
  *   dx, dforget, dgate : [B, T, D] of `dtype`, contiguous; zero in rows of no
  *                        sequence.  dgate is NULL exactly when gate is.
- *   dlower             : [D] fp32 or NULL; needs `partial`, a caller's buffer of
- *                        yuf_gated_scan_partial_rows x D floats (its contents before
- *                        the call do not matter)
+ *   dlower             : [D] fp32 or NULL
  *   dh0                : [B, D] ([n_seqs, D]) fp32 or NULL
+ *   workspace          : as in the forward, always required
  * Every sum has a fixed order: the same call gives the same bits. */
 yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const void* gate,
                                      const void* dy, const int64_t* strides, const float* lower,
                                      const float* h0, const int32_t* cu_seqlens, int n_seqs,
                                      const float* checkpoints, const float* dh_last, void* dx,
                                      void* dforget, void* dgate, float* dlower, float* dh0,
-                                     float* partial, int dtype, int B, int T, int D, void* stream);
+                                     void* workspace, int dtype, int B, int T, int D, void* stream);
 /* One token of B sequences: x, forget, gate (or NULL) [B, D] with row strides
  * strides [3] (NULL = contiguous), y [B, D] contiguous; state [B, D] fp32 with row
  * stride state_stride (>= D) is updated in place, e.g. a slot range of a pool. */

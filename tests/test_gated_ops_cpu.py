@@ -50,14 +50,15 @@ def test_oracle_dropout_words_are_the_published_generator():
 P = 64  # a fake aligned address: the refusals come before any access
 
 
-def _fwd(x=P, f=P, g=P, strides=None, lower=None, h0=None, cu=None, n=0, y=P, last=P, ck=None, dt=0, B=1, T=4, D=8):
-    return _lib.load().yuf_gated_scan_forward(x, f, g, strides, lower, h0, cu, n, y, last, ck, dt, B, T, D, None)
+def _fwd(x=P, f=P, g=P, strides=None, lower=None, h0=None, cu=None, n=0, y=P, last=P, ck=None, ws=P, dt=0, B=1, T=4,
+         D=8):
+    return _lib.load().yuf_gated_scan_forward(x, f, g, strides, lower, h0, cu, n, y, last, ck, ws, dt, B, T, D, None)
 
 
-def _bwd(x=P, f=P, g=P, dy=P, strides=None, cu=None, n=0, ck=P, dx=P, df=P, dg=P, dlower=None, dh0=None, partial=None,
+def _bwd(x=P, f=P, g=P, dy=P, strides=None, cu=None, n=0, ck=P, dx=P, df=P, dg=P, dlower=None, dh0=None, ws=P,
          dt=0, B=1, T=4, D=8):
     return _lib.load().yuf_gated_scan_backward(x, f, g, dy, strides, None, None, cu, n, ck, None, dx, df, dg, dlower,
-                                               dh0, partial, dt, B, T, D, None)
+                                               dh0, ws, dt, B, T, D, None)
 
 
 @pytest.mark.parametrize("kw, word", [
@@ -66,6 +67,7 @@ def _bwd(x=P, f=P, g=P, dy=P, strides=None, cu=None, n=0, ck=P, dx=P, df=P, dg=P
     (dict(cu=P, n=-1), "packed"), (dict(x=None), "required"), (dict(f=None), "required"), (dict(y=None), "required"),
     (dict(x=66), "aligned"), (dict(g=65, dt=1), "aligned"), (dict(y=65, dt=2), "aligned"), (dict(last=66), "aligned"),
     (dict(ck=66), "aligned"), (dict(cu=66, n=1), "aligned"), (dict(lower=66), "aligned"), (dict(h0=66), "aligned"),
+    (dict(ws=None, T=10**6, D=64), "workspace"), (dict(ws=P + 4), "workspace"),
     (dict(strides=(ctypes.c_int64 * 6)(32, -8, 32, 8, 32, 8)), "negative stride"),
 ])
 def test_forward_refuses_on_the_host(kw, word):
@@ -75,7 +77,7 @@ def test_forward_refuses_on_the_host(kw, word):
 
 @pytest.mark.parametrize("kw, word", [
     (dict(dt=7), "type"), (dict(D=-4), "size"), (dict(dy=None), "required"), (dict(dx=None), "required"),
-    (dict(df=None), "required"), (dict(ck=None), "required"), (dict(dg=None), "dgate"), (dict(dlower=P), "partial"),
+    (dict(df=None), "required"), (dict(ck=None), "required"), (dict(dg=None), "dgate"), (dict(ws=None), "workspace"), (dict(ws=P + 8), "workspace"),
     (dict(dx=66), "aligned"), (dict(dg=66), "aligned"), (dict(dh0=66), "aligned"), (dict(cu=P, n=1, B=3), "packed"),
     (dict(strides=(ctypes.c_int64 * 8)(32, 8, 32, 8, 32, 8, -1, 8)), "negative stride"),
 ])
@@ -116,9 +118,12 @@ def test_step_and_dropout_refuse_on_the_host():
 def test_empty_batches_need_no_gpu_and_sizes_are_told():
     lib = _lib.load()
     assert _fwd(B=0, x=None, f=None, y=None) == 0
-    assert [lib.yuf_gated_scan_block(d) for d in (0, 1, 2, 3, -1)] == [8, 16, 16, 0, 0]
-    assert lib.yuf_gated_scan_partial_rows(3, 100, 64, 1) >= 3
-    assert lib.yuf_gated_scan_partial_rows(3, 100, 64, 9) == 0
+    assert [lib.yuf_gated_scan_block(d) > 0 for d in (0, 1, 2)] == [True] * 3
+    assert [lib.yuf_gated_scan_block(d) for d in (3, -1)] == [0, 0]
+    assert lib.yuf_gated_scan_workspace_bytes(3, 100, 64, 1, 1) >= 4 * 3 * 64
+    assert lib.yuf_gated_scan_workspace_bytes(1, 10**6, 64, 1, 0) > 0
+    for bad in [(3, 100, 64, 9), (-1, 100, 64, 0), (3, -1, 64, 0), (3, 100, 0, 0)]:
+        assert lib.yuf_gated_scan_workspace_bytes(*bad, 1) == 0
 
 
 def test_python_callables_refuse_what_is_not_on_the_gpu():

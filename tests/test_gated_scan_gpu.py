@@ -104,7 +104,7 @@ def infer(v):
 
 
 SHAPES = [(1, 1, 1), (2, 7, 33), (3, 16, 64), (1, 17, 2), (2, 129, 40), (1, 300, 130), (2, 1025, 66), (1, 2048, 640),
-          (5, 64, 31), (300, 3, 10)]
+          (5, 64, 31), (300, 3, 10), (1, 1100, 64), (2, 2060, 72), (37, 300, 64), (80, 530, 16), (150, 290, 8)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
@@ -126,7 +126,7 @@ def test_optional_inputs(gate, lower, state):
 
 
 PACKED = [([0, 5, 5, 40, 41, 300], 300), ([0, 0, 0, 64], 64), ([0, 0], 7), ([0, 1, 2, 3], 3), ([0, 128, 256], 256),
-          ([0, 127, 129, 129, 129, 1000], 1100), ([0], 5), ([0, 0, 0], 0), ([0, 700], 700)]
+          ([0, 127, 129, 129, 129, 1000], 1100), ([0], 5), ([0, 0, 0], 0), ([0, 700], 700), ([0, 200, 200, 257, 260], 270)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
@@ -232,8 +232,8 @@ def test_strided_inputs(D, dtype):
     g = torch.autograd.grad((y, last), leaves + [f1], (wide[:, :, 1:D + 1], v["dlast"]))
     full, fg = train(v2)
     check(v2, full, fg)
-    for t, k in zip(g, ("x", "gate", "lower", "state")):
-        assert torch.equal(t, fg[k]), k
+    # another layout may take another kernel, whose sums associate differently
+    check(v2, (y, last), {**dict(zip(("x", "gate", "lower", "state"), g)), "forget": fg["forget"]})
     # the gradient of the shared rows is the sum over the batch, made by autograd in f1's type
     torch.testing.assert_close(g[4], fg["forget"].float().sum(0, keepdim=True).to(g[4].dtype), rtol=2e-2, atol=1e-3)
 

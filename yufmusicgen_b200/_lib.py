@@ -27,7 +27,7 @@ SIGNATURES = {
     "yuf_rosa_forward_compat": [P] * 14 + [I] * 3 + [P],
     "yuf_wkv7_backward": [P] * 15 + [I] * 4 + [P],
     "yuf_rosa_backward": [P] * 16 + [I] * 3 + [P],
-    "yuf_gated_scan_forward": [P, P, P, P, P, P, P, I, P, P, P, I, I, I, I, P],
+    "yuf_gated_scan_forward": [P] * 7 + [I] + [P] * 4 + [I] * 4 + [P],
     "yuf_gated_scan_backward": [P] * 8 + [I] + [P] * 8 + [I] * 4 + [P],
     "yuf_gated_scan_step": [P] * 6 + [ctypes.c_int64, P, I, I, I, P],
     "yuf_dropout": [P, ctypes.c_int64, I, P, ctypes.c_int64, P, I, ctypes.c_int64, ctypes.c_int64, ctypes.c_double,
@@ -118,8 +118,8 @@ def load():
         lib.yuf_wait_timeouts.restype = ctypes.c_uint
         lib.yuf_wait_timeouts.argtypes = []
         lib.yuf_gated_scan_block.argtypes = [I]
-        lib.yuf_gated_scan_partial_rows.restype = ctypes.c_int64
-        lib.yuf_gated_scan_partial_rows.argtypes = [I] * 4
+        lib.yuf_gated_scan_workspace_bytes.restype = ctypes.c_size_t
+        lib.yuf_gated_scan_workspace_bytes.argtypes = [I] * 5
         for name, args in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.argtypes = args

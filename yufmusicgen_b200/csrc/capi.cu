@@ -74,6 +74,7 @@ unsigned int wkv7_decode_wait_timeouts();
 unsigned int gemm_wait_timeouts();
 unsigned int wkv7_rows_wait_timeouts();
 unsigned int wkv7_chunk_tc_wait_timeouts();
+unsigned int gated_scan_wait_timeouts();
 yuf_status_t wkv7_rows(const float* r, const float* w, const float* k, const float* v, const float* a,
                        const float* b, const float* s0, float* y, float* s_out, int B, int T, int H, int N,
                        cudaStream_t st);
@@ -139,8 +140,8 @@ extern "C" {
 unsigned int yuf_wait_timeouts(void) {
   const unsigned int p = yuf::wkv7_pair_wait_timeouts(), d = yuf::wkv7_decode_wait_timeouts(),
                      g = yuf::gemm_wait_timeouts(), r = yuf::wkv7_rows_wait_timeouts(),
-                     c = yuf::wkv7_chunk_tc_wait_timeouts();
-  return (p == ~0u || d == ~0u || g == ~0u || r == ~0u || c == ~0u) ? ~0u : p + d + g + r + c;
+                     c = yuf::wkv7_chunk_tc_wait_timeouts(), s = yuf::gated_scan_wait_timeouts();
+  return (p == ~0u || d == ~0u || g == ~0u || r == ~0u || c == ~0u || s == ~0u) ? ~0u : p + d + g + r + c + s;
 }
 
 yuf_status_t yuf_sync_check(void* stream) {
@@ -377,17 +378,17 @@ static yuf_status_t gated_scan_args(const char* who, const void* const in[4], co
   return YUF_OK;
 }
 
-int yuf_gated_scan_block(int dtype) { return known_dtype(dtype) ? yuf::gated_scan_block(dtype) : 0; }
+int yuf_gated_scan_block(int dtype) { return known_dtype(dtype) ? yuf::GATED_SCAN_BLOCK : 0; }
 
-int64_t yuf_gated_scan_partial_rows(int B, int T, int D, int dtype) {
-  if (!known_dtype(dtype) || B < 0 || T < 0 || D < 1) return 0;
-  return yuf::gated_scan_partial_rows(B, T, D);
+size_t yuf_gated_scan_workspace_bytes(int B, int T, int D, int dtype, int backward) {
+  if (!known_dtype(dtype) || B < 0 || T < 0 || T > (1 << 30) || D < 1) return 0;
+  return yuf::gated_scan_workspace_floats(B, T, D, dtype, backward != 0) * sizeof(float);
 }
 
 yuf_status_t yuf_gated_scan_forward(const void* x, const void* forget, const void* gate, const int64_t* strides,
                                     const float* lower, const float* h0, const int32_t* cu_seqlens, int n_seqs,
-                                    void* y, float* h_last, float* checkpoints, int dtype, int B, int T, int D,
-                                    void* stream) {
+                                    void* y, float* h_last, float* checkpoints, void* workspace, int dtype, int B,
+                                    int T, int D, void* stream) {
   g_err[0] = 0;
   yuf::GatedScanArgs a;
   const void* in[4] = {x, forget, gate, nullptr};
@@ -398,7 +399,10 @@ yuf_status_t yuf_gated_scan_forward(const void* x, const void* forget, const voi
   REQUIRE(aligned(y, dtype_size(dtype)) && aligned(h_last, 4) && aligned(checkpoints, 4),
           "gated scan: an output is not aligned to its elements");
   if (B == 0) return YUF_OK;
-  a.y = y; a.h_last = h_last; a.ckpt = checkpoints;
+  REQUIRE(workspace || yuf::gated_scan_workspace_floats(B, T, D, dtype, false) == 0,
+          "gated scan: this size needs a workspace");
+  REQUIRE(aligned(workspace, 16), "gated scan: the workspace is not 16-byte aligned");
+  a.y = y; a.h_last = h_last; a.ckpt = checkpoints; a.work = static_cast<float*>(workspace);
   return yuf::gated_scan_forward(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -406,7 +410,7 @@ yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const vo
                                      const int64_t* strides, const float* lower, const float* h0,
                                      const int32_t* cu_seqlens, int n_seqs, const float* checkpoints,
                                      const float* dh_last, void* dx, void* dforget, void* dgate, float* dlower,
-                                     float* dh0, float* partial, int dtype, int B, int T, int D, void* stream) {
+                                     float* dh0, void* workspace, int dtype, int B, int T, int D, void* stream) {
   g_err[0] = 0;
   yuf::GatedScanArgs a;
   const void* in[4] = {x, forget, gate, dy};
@@ -416,10 +420,11 @@ yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const vo
   REQUIRE((long long)B * T == 0 || (dy && dx && dforget && checkpoints),
           "gated scan backward: dy, dx, dforget and checkpoints are required");
   REQUIRE((long long)B * T == 0 || !gate || dgate, "gated scan backward: dgate is required with a gate");
-  REQUIRE(B == 0 || !dlower || partial, "gated scan backward: dlower needs the partial buffer");
+  REQUIRE(B == 0 || workspace, "gated scan backward: the workspace is required");
+  REQUIRE(aligned(workspace, 16), "gated scan backward: the workspace is not 16-byte aligned");
   const size_t e = dtype_size(dtype);
   REQUIRE(aligned(dx, e) && aligned(dforget, e) && aligned(dgate, e) && aligned(dlower, 4) && aligned(dh0, 4) &&
-              aligned(partial, 4) && aligned(checkpoints, 4) && aligned(dh_last, 4),
+              aligned(checkpoints, 4) && aligned(dh_last, 4),
           "gated scan backward: a buffer is not aligned to its elements");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (B == 0) {
@@ -429,7 +434,7 @@ yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const vo
   }
   a.ckpt = const_cast<float*>(checkpoints); a.dh_last = dh_last;
   a.dx = dx; a.df = dforget; a.dg = gate ? dgate : nullptr;
-  a.dlower = dlower; a.dh0 = dh0; a.partial = dlower ? partial : nullptr;
+  a.dlower = dlower; a.dh0 = dh0; a.work = static_cast<float*>(workspace);
   return yuf::gated_scan_backward(a, s);
 }
 

@@ -19,13 +19,14 @@ struct GatedScanArgs {
   // backward
   const float* dh_last;                              // NULL = zeros
   void *dx, *df, *dg;
-  float *dlower, *dh0, *partial;
+  float *dlower, *dh0;
+  float* partial;                                    // set from work by the dispatch
+  float* work;                                       // gated_scan_workspace_floats
 };
 
-// tokens between two saved states, by element type
-constexpr int gated_scan_block(int dtype) { return dtype == YUF_DTYPE_F32 ? 8 : 16; }
-// rows of `partial` the backward writes
-long long gated_scan_partial_rows(int B, int T, int D);
+// tokens between two saved states
+constexpr int GATED_SCAN_BLOCK = 16;
+size_t gated_scan_workspace_floats(int B, int T, int D, int dtype, bool backward);
 
 yuf_status_t gated_scan_forward(const GatedScanArgs& a, cudaStream_t st);
 yuf_status_t gated_scan_backward(const GatedScanArgs& a, cudaStream_t st);

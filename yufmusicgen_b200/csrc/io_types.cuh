@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace yuf {
@@ -13,13 +15,14 @@ struct Fv {
   float v[V];
 };
 
+// each operation rounds by itself (no contraction), whatever kernel it stands in
 YUF_DEVICE float2 as2(const Fv<2>& a) { return make_float2(a.v[0], a.v[1]); }
 YUF_DEVICE Fv<2> of2(float2 a) { return Fv<2>{{a.x, a.y}}; }
-YUF_DEVICE Fv<1> mul(Fv<1> a, Fv<1> b) { return Fv<1>{{a.v[0] * b.v[0]}}; }
+YUF_DEVICE Fv<1> mul(Fv<1> a, Fv<1> b) { return Fv<1>{{__fmul_rn(a.v[0], b.v[0])}}; }
 YUF_DEVICE Fv<2> mul(Fv<2> a, Fv<2> b) { return of2(fmul2(as2(a), as2(b))); }
 YUF_DEVICE Fv<1> fma(Fv<1> a, Fv<1> b, Fv<1> c) { return Fv<1>{{fmaf(a.v[0], b.v[0], c.v[0])}}; }
 YUF_DEVICE Fv<2> fma(Fv<2> a, Fv<2> b, Fv<2> c) { return of2(ffma2(as2(a), as2(b), as2(c))); }
-YUF_DEVICE Fv<1> add(Fv<1> a, Fv<1> b) { return Fv<1>{{a.v[0] + b.v[0]}}; }
+YUF_DEVICE Fv<1> add(Fv<1> a, Fv<1> b) { return Fv<1>{{__fadd_rn(a.v[0], b.v[0])}}; }
 YUF_DEVICE Fv<2> add(Fv<2> a, Fv<2> b) { return of2(__fadd2_rn(as2(a), as2(b))); }
 template <int V>
 YUF_DEVICE Fv<V> splat(float x) {
@@ -102,13 +105,13 @@ YUF_DEVICE void store_f32(float* p, Fv<V> f) {
 }
 
 // sigmoid(x) and sigmoid(-x) = 1 - sigmoid(x), both to fp32 relative accuracy:
-// e = 2^min(-x log2 e, 126), s = 1 / (1 + e), 1 - s = e s.  The cap keeps e s
-// finite for very negative x; NaN goes through.
-YUF_DEVICE float sigmoid_exp(float x) {
-  float z = x * -1.4426950408889634f, e;
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(126.f));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z));
-  return e;
+// e = 2^(-x log2 e), s = 1 / (1 + e), 1 - s = e s.  x is kept from below
+// SIGMOID_MIN, where e would overflow and e s be inf * 0; NaN goes through.
+constexpr float SIGMOID_MIN = -87.f;  // exact in bf16 and fp16
+YUF_DEVICE float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 YUF_DEVICE float rcp_fast(float x) {
   float r;
@@ -116,20 +119,56 @@ YUF_DEVICE float rcp_fast(float x) {
   return r;
 }
 template <int V>
+YUF_DEVICE Fv<V> sigmoid_exp(Fv<V> x) {
+  Fv<V> z = mul(x, splat<V>(-1.4426950408889634f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) z.v[i] = exp2_fast(z.v[i]);
+  return z;
+}
+template <int V>
+YUF_DEVICE Fv<V> rcp_1p(Fv<V> e) {
+  Fv<V> d = add(e, splat<V>(1.f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) d.v[i] = rcp_fast(d.v[i]);
+  return d;
+}
+// of x >= SIGMOID_MIN
+template <int V>
 YUF_DEVICE void sigmoid_pair(Fv<V> x, Fv<V>& s, Fv<V>& one_minus_s) {
-  Fv<V> e;
-#pragma unroll
-  for (int i = 0; i < V; ++i) e.v[i] = sigmoid_exp(x.v[i]);
-  const Fv<V> d = add(e, splat<V>(1.f));
-#pragma unroll
-  for (int i = 0; i < V; ++i) s.v[i] = rcp_fast(d.v[i]);
+  const Fv<V> e = sigmoid_exp(x);
+  s = rcp_1p(e);
   one_minus_s = mul(e, s);
 }
 template <int V>
-YUF_DEVICE Fv<V> sigmoid_of(Fv<V> x) {
-  Fv<V> s, t;
-  sigmoid_pair(x, s, t);
-  return s;
+YUF_DEVICE Fv<V> sigmoid_of(Fv<V> x) {  // any x
+  return rcp_1p(sigmoid_exp(x));
+}
+// max(x, SIGMOID_MIN) that keeps NaN, on the elements as they lie in memory
+template <typename T, int V>
+YUF_DEVICE Raw<T, V> sigmoid_arg(Raw<T, V> x) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 1) {
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.r) : "f"(SIGMOID_MIN));
+    } else {
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.r.x) : "f"(SIGMOID_MIN));
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.r.y) : "f"(SIGMOID_MIN));
+    }
+  } else if constexpr (V == 2) {
+    if constexpr (std::is_same_v<T, __half>) {
+      const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&x.r), __float2half2_rn(SIGMOID_MIN));
+      x.r = *reinterpret_cast<const unsigned*>(&m);
+    } else {
+      const __nv_bfloat162 m =
+          __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&x.r), __float2bfloat162_rn(SIGMOID_MIN));
+      x.r = *reinterpret_cast<const unsigned*>(&m);
+    }
+  } else {
+    if constexpr (std::is_same_v<T, __half>)
+      x.r = __half_as_ushort(__hmax_nan(__ushort_as_half(x.r), __float2half_rn(SIGMOID_MIN)));
+    else
+      x.r = __bfloat16_as_ushort(__hmax_nan(__ushort_as_bfloat16(x.r), __float2bfloat16_rn(SIGMOID_MIN)));
+  }
+  return x;
 }
 
 }  // namespace yuf

@@ -75,6 +75,12 @@ def _check(x, forget, gate, lower, state, cu_seqlens):
     return rows
 
 
+def _workspace(x, dtype, backward):
+    """Device scratch of one call, or None where it needs none."""
+    n = _lib.load().yuf_gated_scan_workspace_bytes(*x.shape, dtype, backward)
+    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
 def _forward(x, forget, gate, lower, state, cu, rows, save):
     """The kernel call on checked tensors with unit rows; ``(y, final_state, checkpoints)``."""
     B, T, D = x.shape
@@ -85,11 +91,12 @@ def _forward(x, forget, gate, lower, state, cu, rows, save):
     if save:
         block = _lib.load().yuf_gated_scan_block(dtype)
         ckpt = torch.empty((B, (T + block - 1) // block, D), dtype=torch.float32, device=x.device)
+    work = _workspace(x, dtype, 0)
     strides = _Strides6(x.stride(0), x.stride(1), forget.stride(0), forget.stride(1),
                         *((0, 0) if gate is None else (gate.stride(0), gate.stride(1))))
     call_on(x.device, "yuf_gated_scan_forward", x.data_ptr(), forget.data_ptr(), _lib.ptr(gate), strides,
             _lib.ptr(lower), _lib.ptr(state), _lib.ptr(cu), 0 if cu is None else rows, y.data_ptr(), last.data_ptr(),
-            _lib.ptr(ckpt), dtype, B, T, D)
+            _lib.ptr(ckpt), _lib.ptr(work), dtype, B, T, D)
     return y, last, ckpt
 
 
@@ -112,10 +119,10 @@ class _GatedScan(torch.autograd.Function):
         dlast = None if dlast is None else dlast.contiguous()
         dx, df, dg = (None if t is None else torch.empty((B, T, D), dtype=x.dtype, device=x.device)
                       for t in (x, forget, gate))
-        dlower = partial = dstate = None
+        dlower = dstate = None
         if lower is not None and ctx.needs_input_grad[3]:
             dlower = torch.empty_like(lower)
-            partial = torch.empty((_lib.load().yuf_gated_scan_partial_rows(B, T, D, dtype), D), device=x.device)
+        work = _workspace(x, dtype, 1)
         if state is not None and ctx.needs_input_grad[4]:
             dstate = torch.empty((ctx.rows, D), device=x.device)
         strides = _Strides8(x.stride(0), x.stride(1), forget.stride(0), forget.stride(1),
@@ -124,7 +131,7 @@ class _GatedScan(torch.autograd.Function):
         call_on(x.device, "yuf_gated_scan_backward", x.data_ptr(), forget.data_ptr(), _lib.ptr(gate), dy.data_ptr(),
                 strides, _lib.ptr(lower), _lib.ptr(state), _lib.ptr(cu), 0 if cu is None else ctx.rows,
                 ckpt.data_ptr(), _lib.ptr(dlast), dx.data_ptr(), df.data_ptr(), _lib.ptr(dg), _lib.ptr(dlower),
-                _lib.ptr(dstate), _lib.ptr(partial), dtype, B, T, D)
+                _lib.ptr(dstate), _lib.ptr(work), dtype, B, T, D)
         return dx, df, dg, dlower, dstate, None, None
 
 
