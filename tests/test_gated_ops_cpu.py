@@ -12,7 +12,8 @@ torch = pytest.importorskip("torch")
 from oracle import gated  # noqa: E402
 from oracle.philox import philox4x32_10  # noqa: E402
 from yufmusicgen_b200 import _lib  # noqa: E402
-from yufmusicgen_b200.dropout import _row_stride, dropout  # noqa: E402
+from yufmusicgen_b200._torch import ops  # noqa: E402
+from yufmusicgen_b200.dropout import dropout  # noqa: E402
 from yufmusicgen_b200.gated_scan import gated_scan, gated_scan_step  # noqa: E402
 
 
@@ -136,17 +137,26 @@ def test_python_callables_refuse_what_is_not_on_the_gpu():
         gated_scan_step(x[0], x[0], x[0])
     with pytest.raises(ValueError, match="CUDA"):
         dropout(x, 0.1, 1)
+    for bad in (None, 3, "x", [1.0]):
+        with pytest.raises(TypeError, match="tensor"):
+            gated_scan(bad, x)
+        with pytest.raises(TypeError, match="tensor"):
+            gated_scan(x, x if bad is None else bad, bad if bad is not None else 5)
+        with pytest.raises((TypeError, ValueError)):
+            dropout(bad, 0.1, 1)
+        with pytest.raises(TypeError):
+            ops.gated_scan(x, bad)
 
 
 def test_row_strides():
     """The row stride that dropout's kernel is given, or None where rows have none."""
     t = torch.zeros(4, 6, 10)
-    assert _row_stride(t) == 10
-    assert _row_stride(t[:, :, 2:5]) == 10
-    assert _row_stride(t[:, 1:3]) is None            # two strides
-    assert _row_stride(t[:, 1:2, :4]) == 60          # axes of one row are not rows
-    assert _row_stride(t[0, 0]) == 10 and _row_stride(t[0, 0, 2:5]) == 3
-    assert _row_stride(t.transpose(1, 2)) is None
-    assert _row_stride(t[:, :, :1]) == 10
-    assert _row_stride(torch.zeros(1, 1, 8).expand(4, 6, 8)) == 0
-    assert _row_stride(torch.zeros(1, 6, 8).expand(4, 6, 8)) is None
+    assert ops.row_stride(t) == 10
+    assert ops.row_stride(t[:, :, 2:5]) == 10
+    assert ops.row_stride(t[:, 1:3]) is None            # two strides
+    assert ops.row_stride(t[:, 1:2, :4]) == 60          # axes of one row are not rows
+    assert ops.row_stride(t[0, 0]) == 10 and ops.row_stride(t[0, 0, 2:5]) == 3
+    assert ops.row_stride(t.transpose(1, 2)) is None
+    assert ops.row_stride(t[:, :, :1]) == 10
+    assert ops.row_stride(torch.zeros(1, 1, 8).expand(4, 6, 8)) == 0
+    assert ops.row_stride(torch.zeros(1, 6, 8).expand(4, 6, 8)) is None

@@ -1,4 +1,5 @@
-"""Build recipe for ``libyufb200.so`` (sm_100a only).
+"""Build recipe for ``libyufb200.so`` (sm_100a only) and ``_yuf_torch.so``, the
+Python module that calls it on torch tensors.
 
 Each ``csrc/*.cu`` / ``*.cpp`` file is compiled to an object under
 ``yufmusicgen_b200/_build/`` (in parallel, skipped when up to date) and linked
@@ -9,16 +10,20 @@ travels with the checkout.  ``python -m yufmusicgen_b200.build [-v]``.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_build"
 LIB = PKG / "libyufb200.so"
+TORCH_SRC = CSRC / "torch" / "binding.cpp"
+TORCH_MODULE = PKG / "_yuf_torch.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -56,11 +61,50 @@ def _compile(src: Path, ptxas_verbose: bool) -> tuple[Path, str]:
     return obj, p.stderr
 
 
+def _torch_dir() -> Path:
+    spec = importlib.util.find_spec("torch")  # found, not imported
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch not found; it is required to build _yuf_torch")
+    return Path(spec.origin).parent
+
+
+def _compile_torch() -> Path:
+    """Compile the torch module's object (it is linked once the library is there)."""
+    obj = OUT_DIR / "torch_binding.o"
+    torch_dir = _torch_dir()
+    newest = max(TORCH_SRC.stat().st_mtime, (INCLUDE / "yufb200.h").stat().st_mtime,
+                 (torch_dir / "version.py").stat().st_mtime)
+    if obj.exists() and obj.stat().st_mtime >= newest:
+        return obj
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-I", str(INCLUDE), "-isystem", str(torch_dir / "include"),
+           "-isystem", str(torch_dir / "include/torch/csrc/api/include"), "-I", sysconfig.get_paths()["include"],
+           "-isystem", str(cuda / "include"), "-c", str(TORCH_SRC), "-o", str(obj)]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"g++ failed on {TORCH_SRC.name}:\n{p.stdout}\n{p.stderr}")
+    return obj
+
+
+def _link_torch(obj: Path) -> None:
+    if TORCH_MODULE.exists() and TORCH_MODULE.stat().st_mtime >= obj.stat().st_mtime:
+        return
+    tmp = TORCH_MODULE.with_suffix(".so.tmp")
+    cmd = ["g++", "-shared", "-o", str(tmp), str(obj), "-L", str(PKG), "-lyufb200", "-Wl,-rpath,$ORIGIN",
+           "-L", str(_torch_dir() / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"link of {TORCH_MODULE.name} failed:\n{p.stdout}\n{p.stderr}")
+    os.replace(tmp, TORCH_MODULE)
+
+
 def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        torch_obj = ex.submit(_compile_torch)
         results = list(ex.map(lambda s: _compile(s, ptxas_verbose), srcs))
+        torch_obj = torch_obj.result()
     objs = [o for o, _ in results]
     if verbose:
         for o, log in results:
@@ -74,6 +118,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n{p.stdout}\n{p.stderr}")
         os.replace(tmp, LIB)
+    _link_torch(torch_obj)
     return LIB
 
 
