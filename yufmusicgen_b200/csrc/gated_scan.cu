@@ -360,11 +360,23 @@ YUF_DEVICE const T* row_ptr(const void* t, long long sb, int b, int c) {
   return static_cast<const T*>(t) + b * sb + c;
 }
 
+// 1 / (1 + e) of token u: every other pair of channels on the FMA pipe (see
+// rcp_1p_newton), which balances the two units.
+template <int V>
+YUF_DEVICE Fv<V> rcp_turns(Fv<V> e, int u) {
+  if constexpr (V == 2)
+    if (u & 1) return rcp_1p_newton(e);
+  return rcp_1p(e);
+}
 // Rates of a group of tokens, and gates of a group.
 template <typename T, int V, int N>
 YUF_DEVICE void group_pairs(const Raw<T, V> (&f)[N], Fv<V> (&s)[N], Fv<V> (&m)[N]) {
 #pragma unroll
-  for (int u = 0; u < N; ++u) sigmoid_pair(sigmoid_arg(f[u]).get(), s[u], m[u]);
+  for (int u = 0; u < N; ++u) {
+    m[u] = sigmoid_exp(sigmoid_arg(f[u]).get());
+    s[u] = rcp_turns(m[u], u);
+    m[u] = mul(m[u], s[u]);
+  }
 }
 template <typename T, int V, int N>
 YUF_DEVICE void group_rates(const Columns<T, V>& k, const Raw<T, V> (&f)[N], Fv<V> (&a)[N], Fv<V> (&in)[N]) {
@@ -378,7 +390,7 @@ YUF_DEVICE void group_rates(const Columns<T, V>& k, const Raw<T, V> (&f)[N], Fv<
 template <typename T, int V, int N>
 YUF_DEVICE void group_gates(const Raw<T, V> (&g)[N], Fv<V> (&s)[N]) {
 #pragma unroll
-  for (int u = 0; u < N; ++u) s[u] = sigmoid_of(g[u].get());
+  for (int u = 0; u < N; ++u) s[u] = rcp_turns(sigmoid_exp(sigmoid_arg(g[u]).get()), u);
 }
 
 // ---------------------------------------------------------------------------

@@ -143,6 +143,22 @@ template <int V>
 YUF_DEVICE Fv<V> sigmoid_of(Fv<V> x) {  // any x
   return rcp_1p(sigmoid_exp(x));
 }
+// The same reciprocal on the FMA pipe, for kernels whose exponentials and reciprocals
+// keep the special function unit busy: 1 / u of a float is near K - bits(u) read as a
+// float (the exponent negated, the mantissa on a line; K minimises the largest error
+// over [1, 4): 5.05e-2), then Newton's iteration with e = 1 - u r, once to third order
+// (r + r (e + e^2): 1.3e-4) and once to second: 1.3 x 2^-24 with roundings.  d = -u =
+// -(1 + e^-x), so that e is one FMA; u <= 2^126.
+YUF_DEVICE Fv<2> rcp_1p_newton(Fv<2> ex) {
+  const Fv<2> one = splat<2>(1.f), d = fma(ex, splat<2>(-1.f), splat<2>(-1.f));
+  Fv<2> r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r.v[i] = __uint_as_float(0xFEF311C0u - __float_as_uint(d.v[i]));
+  Fv<2> e = fma(d, r, one);
+  r = fma(r, fma(e, e, e), r);
+  e = fma(d, r, one);
+  return fma(r, e, r);
+}
 // max(x, SIGMOID_MIN) that keeps NaN, on the elements as they lie in memory
 template <typename T, int V>
 YUF_DEVICE Raw<T, V> sigmoid_arg(Raw<T, V> x) {
