@@ -566,7 +566,10 @@ YUF_DEVICE int range_start(const Split& sp) {
 }
 YUF_DEVICE int range_runs(const Split& sp, int t, int T) { return max(0, min(sp.runs, (T - t + L - 1) / L)); }
 
-// The map of each range, forward: x and f; two stages.
+// The map of each range, forward: x and f; two stages.  The range is walked from its
+// end, H = sum_j (a_{j+1} ... a_last) i_j x_j, so that what the ranges kernel reads
+// first was read last here and is still in L2.  (The backward's are the other way
+// round by themselves.)
 template <typename T, int V, bool PACKED, bool TMA>
 __global__ void __launch_bounds__(32 * NW_MAX)
     gated_scan_forward_maps_kernel(const GatedScanArgs p, const __grid_constant__ ScanMaps tm, const Split sp) {
@@ -581,12 +584,13 @@ __global__ void __launch_bounds__(32 * NW_MAX)
   const int r0 = range_start(sp), n = range_runs(sp, r0, p.T);
   char* const mine = smem + w * (4 * SLOT);
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + nw * 4 * SLOT) + 2 * w;
+  const auto t_of = [&](int i) { return r0 + (n - 1 - i) * L; };
   const auto issue = [&](int i) {  // by lane 0
     if (i >= n) return;
     char* const s = mine + (i & 1) * 2 * SLOT;
     mbar_expect_tx(&full[i & 1], 2 * SLOT);
-    box_load(s, &tm.x, &full[i & 1], k.c0, r0 + i * L, k.b);
-    box_load(s + SLOT, &tm.f, &full[i & 1], k.c0, r0 + i * L, k.b);
+    box_load(s, &tm.x, &full[i & 1], k.c0, t_of(i), k.b);
+    box_load(s + SLOT, &tm.f, &full[i & 1], k.c0, t_of(i), k.b);
   };
   if constexpr (TMA) {
     if (lane == 0) {
@@ -601,8 +605,9 @@ __global__ void __launch_bounds__(32 * NW_MAX)
   }
   Run run{};
   Fv<V> A = splat<V>(1.f), H = splat<V>(0.f);
+  bool cut = false;  // before a first token nothing reaches the range's end any more
   for (int i = 0; i < n; ++i) {
-    const int t0 = r0 + i * L;
+    const int t0 = t_of(i);
     char* const sx = mine + (i & 1) * 2 * SLOT;
     Raw<T, V> xr[TMA ? 1 : L], fr[TMA ? 1 : L];
     const auto X = [&](int j) { return row_at<TMA, T, V>(sx, xr, j, lane); };
@@ -614,36 +619,34 @@ __global__ void __launch_bounds__(32 * NW_MAX)
     }
     look<PACKED>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
-    if (run.plain()) {
+    if (PACKED && cut) {
+    } else if (run.plain()) {
 #pragma unroll
-      for (int j0 = 0; j0 < L; j0 += GROUP) {
+      for (int j0 = L - GROUP; j0 >= 0; j0 -= GROUP) {
         Raw<T, V> xv[GROUP], fv[GROUP];
         Fv<V> a[GROUP], in[GROUP];
         take(xv, X, j0);
         take(fv, F, j0);
         group_rates(k, fv, a, in);
 #pragma unroll
-        for (int u = 0; u < GROUP; ++u) {
-          H = fma(a[u], H, mul(in[u], xv[u].get()));
+        for (int u = GROUP - 1; u >= 0; --u) {
+          H = fma(A, mul(in[u], xv[u].get()), H);
           A = mul(A, a[u]);
         }
-#pragma unroll
-        for (int u = 0; u < V; ++u)
-          if (PACKED && signbit(A.v[u])) A.v[u] = CUT;  // a cut stays one, also where a is 0
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        if (run.live >> j & 1) {
+      for (int j = L - 1; j >= 0; --j) {
+        if ((run.live >> j & 1) && !(PACKED && cut)) {
           Fv<V> a, in;
           k.rates(F(j), a, in);
-          Fv<V> bx = mul(in, X(j).get());
+          H = fma(A, mul(in, X(j).get()), H);
+          A = mul(A, a);
           if (run.first >> j & 1) {
-            const Fv<V> h0 = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
-            if (p.h0) bx = fma(a, h0, bx);
-            a = splat<V>(CUT);
+            if (p.h0) H = fma(A, row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act), H);
+            A = splat<V>(CUT);
+            cut = true;
           }
-          compose<PACKED>(A, H, a, bx);
         }
       }
     }
@@ -1176,8 +1179,12 @@ __global__ void __launch_bounds__(32 * NW_MAX)
         }
       }
     };
-    if (run.plain() && !(PACKED && cut)) pass(std::true_type{});
-    else pass(std::false_type{});
+    if (PACKED && cut) {
+    } else if (run.plain()) {
+      pass(std::true_type{});
+    } else {
+      pass(std::false_type{});
+    }
     if constexpr (TMA) {
       __syncwarp();
       if (lane == 0) issue(i + 2);
