@@ -151,6 +151,13 @@ def test_captured_graph_draws_new_masks():
         assert torch.equal(y, want) and torch.equal(dx, torch.autograd.grad(want, x, dy)[0])
 
 
+def test_gradients_are_not_differentiable_themselves():
+    x = rnd((8, 8), torch.float32, 9).requires_grad_(True)
+    (gx,) = torch.autograd.grad((dropout(x, 0.5, 1) ** 2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable themselves"):
+        gx.sum().backward()
+
+
 def test_refusals():
     x = torch.zeros(4, 8, device=DEV)
     for err, word, kw in [

@@ -178,6 +178,34 @@ def test_packed_equals_each_sequence_alone_and_shields_it():
     assert torch.equal(grads["x"][:, 37:300, 1:], cgrads["x"][:, 37:300, 1:])
 
 
+def test_a_short_packed_row_shields_its_sequences():
+    """As above at a length where one block walks the whole row, the cut inside a warp's tokens
+    and at a warp's first."""
+    cu = [0, 21, 48, 150]
+    v = make(1, 160, 48, "bf16", cu=cu, seed=30)
+    clean, cgrads = train(v)
+    v["x"][0, 20], v["x"][0, 47] = float("inf"), float("-inf")
+    for k in ("x", "forget", "gate", "dy"):
+        v[k][:, 150:] = float("nan")
+    got, grads = train(v)
+    assert torch.equal(got[0][:, 48:], clean[0][:, 48:]) and torch.equal(got[1][2], clean[1][2])
+    assert torch.isinf(got[1][:2]).all() and torch.equal(got[0][:, 21:47], clean[0][:, 21:47])
+    for k in ("x", "forget", "gate"):
+        assert torch.equal(grads[k][:, 48:], cgrads[k][:, 48:]), k
+    assert torch.equal(grads["state"][2], cgrads["state"][2])
+
+
+def test_gradients_are_not_differentiable_themselves():
+    v = make(1, 20, 8, "fp32", seed=31)
+    x, w = v["x"].clone().requires_grad_(True), torch.ones(8, device=DEV, requires_grad=True)
+    y, _ = gated_scan(x * w, v["forget"])
+    (gx,) = torch.autograd.grad(y.sum(), x, create_graph=True)   # allowed: a graph around the operator
+    check_x, = torch.autograd.grad(gated_scan(x * w, v["forget"])[0].sum(), x)
+    assert torch.equal(gx, check_x)
+    with pytest.raises(RuntimeError, match="not differentiable themselves"):
+        gx.sum().backward()
+
+
 def test_a_channel_of_nan_stays_alone():
     v = make(2, 200, 6, "bf16", seed=10)
     clean, cg = train(v)

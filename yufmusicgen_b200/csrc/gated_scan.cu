@@ -123,11 +123,20 @@ struct Place {
   unsigned long long limit;  // bound of each wait, ns; cut short once one has expired
 };
 
-// A wait that gave up: count it, and do not wait as long again.
+// A wait that gave up: count it, and do not wait as long again (the results are void,
+// yuf_sync_check says so).
 YUF_DEVICE void check_wait(Place& q, bool ok) {
   if (__all_sync(0xffffffffu, ok)) return;
   if (q.lane == 0 && q.limit == WAIT_NS) atomicAdd(&g_gated_wait_timeouts, 1u);
   q.limit = 1000;
+}
+
+// The end of a kernel in which a wait gave up: its copies get time to land before the
+// block's shared memory is given away.
+YUF_DEVICE void linger(const Place& q) {
+  if (q.limit == WAIT_NS) return;
+  const unsigned long long t0 = global_ns();
+  while (global_ns() - t0 < 10ull * 1000 * 1000) __nanosleep(1000);
 }
 
 // Shared memory of the exchange between a block's warps: two copies of each (a
@@ -546,6 +555,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
   }
   if (!PACKED && p.h_last && w == nw - 1 && k.act) store_f32<V>(p.h_last + (long long)k.b * p.D + k.c, h);
   if (TMA && lane == 0) bulk_wait_read<0>();
+  if constexpr (TMA) linger(at);
 }
 
 // ---------------------------------------------------------------------------
@@ -656,6 +666,7 @@ __global__ void __launch_bounds__(32 * NW_MAX)
     }
   }
   leave_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), A, H);
+  if constexpr (TMA) linger(at);
 }
 
 // Each range from its true start state, in one pass.  Two stages of x, f, g; y is
@@ -772,6 +783,7 @@ __global__ void __launch_bounds__(32 * NW_MAX)
   // the range that holds the last token
   if (!PACKED && p.h_last && n > 0 && r0 + n * L >= p.T && k.act)
     store_f32<V>(p.h_last + (long long)k.b * p.D + k.c, h);
+  if constexpr (TMA) linger(at);
 }
 
 // ---------------------------------------------------------------------------
@@ -1083,6 +1095,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
   if (!PACKED && p.dh0 && k.act && (RANGES ? r0 == 0 : w == 0)) store_f32<V>(p.dh0 + (long long)k.b * p.D + k.c, G);
   if (p.partial) write_partial<V>(joint, p, at, dlo, (long long)k.b * sp.chunks + blockIdx.x % sp.chunks, k.c, k.act);
   if (OUT_SLOT && lane == 0) bulk_wait_read<0>();
+  if constexpr (TMA) linger(at);
 }
 
 // The map of each range, backward: f, dy and g; two stages.  h is not needed.
@@ -1191,6 +1204,7 @@ __global__ void __launch_bounds__(32 * NW_MAX)
     }
   }
   leave_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), A, H);
+  if constexpr (TMA) linger(at);
 }
 
 // dlower[c] = sum over rows of partial[rows, D], in a fixed order

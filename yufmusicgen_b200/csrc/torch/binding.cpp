@@ -4,6 +4,7 @@
 // its current stream.  In C++ because the smallest calls are bound by the host: a
 // training call through a Python autograd function took 160 us, 100 of it Python.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -69,6 +70,16 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 // A failing library call (the message of its thread).
 void check(const char* name, yuf_status_t st) {
   TORCH_CHECK(st == YUF_OK, name, " failed with ", yuf_status_string(st), ": ", yuf_last_error());
+}
+// Gradients made while a graph of the backward is recorded (create_graph): they may be
+// used, but an attempt to differentiate through them is an error.
+variable_list once(const char* name, bool recorded, variable_list grads) {
+  if (!recorded) return grads;
+  for (Tensor& t : grads)
+    if (t.defined())
+      t = torch::autograd::DelayedError(std::string(name) + ": the gradients are not differentiable themselves", 1)
+              .apply({t.detach().set_requires_grad(true)})[0];
+  return grads;
 }
 // The tensors' device for as long as a call lasts, and its current stream.
 struct On {
@@ -163,7 +174,8 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     return {out[0], out[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "gated_scan: the gradients are not differentiable themselves");
+    const bool recorded = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
     const auto saved = ctx->get_saved_variables();
     const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], dtype_of(saved[0]),
                     ctx->saved_data["rows"].toInt()};
@@ -187,7 +199,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
                                   ptr<float>(saved[6]), ptr<float>(dlast), ptr<void>(dx), ptr<void>(df), ptr<void>(dg),
                                   ptr<float>(dlower), ptr<float>(dstate), ptr<void>(work), in.dtype, in.B(), in.T(),
                                   in.D(), on.stream));
-    return {dx, df, dg, dlower, dstate, Tensor(), Tensor()};
+    return once("gated_scan", recorded, {dx, df, dg, dlower, dstate, Tensor(), Tensor()});
   }
 };
 
@@ -241,7 +253,8 @@ struct Dropout : torch::autograd::Function<Dropout> {
     return drop(x, r, Draw{p, (uint64_t)seed, (uint64_t)step}, step_t, r.defined() ? r.scalar_type() : x.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "dropout: the gradients are not differentiable themselves");
+    const bool recorded = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
     const auto draw = ctx->saved_data["draw"].toIntVector();
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
@@ -249,7 +262,9 @@ struct Dropout : torch::autograd::Function<Dropout> {
     if (dy.defined() && ctx->needs_input_grad(0))
       dx = drop(dy, Tensor(), Draw{ctx->saved_data["p"].toDouble(), (uint64_t)draw[0], (uint64_t)draw[1]},
                 saved.empty() ? Tensor() : saved[0], (at::ScalarType)draw[2]);
-    return {dx, ctx->saved_data["residual"].toBool() ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor dr = ctx->saved_data["residual"].toBool() ? dy : Tensor();
+    dx = once("dropout", recorded, {dx})[0];  // dr is dy, with its own history
+    return {dx, dr, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 

@@ -17,7 +17,8 @@ Per channel of ``[B, T, D]``, in fp32 inside whatever the tensors' type::
 ``x``, ``forget`` and ``gate`` are float32, bfloat16 or float16 and may be column
 ranges of one projection (any batch and token strides).  ``lower`` and ``state``
 are float32.  Calls run on the tensors' device and its current stream, and may be
-captured in CUDA graphs, their backward passes too.
+captured in CUDA graphs, their backward passes too (as ever with torch, while no
+eager graph of the same leaves is alive).
 """
 
 from __future__ import annotations
@@ -36,8 +37,8 @@ def gated_scan(x, forget, gate=None, lower=None, state=None, cu_seqlens=None):
     rows behind the last sequence play no part; their ``y`` and gradients are 0.
     The contents of ``cu_seqlens`` are not checked (that would wait for the GPU).
 
-    Raises ValueError or TypeError for what the kernels do not take; gradients
-    cannot be differentiated again (RuntimeError)."""
+    Raises ValueError or TypeError for what the kernels do not take.  The gradients
+    cannot be differentiated again (RuntimeError where that is tried)."""
     return ops.gated_scan(x, forget, gate, lower, state, cu_seqlens)
 
 
