@@ -26,6 +26,26 @@ struct GatedScanArgs {
 
 // tokens between two saved states
 constexpr int GATED_SCAN_BLOCK = 16;
+constexpr int GATED_SCAN_WARPS = 16;  // warps per block, at most
+
+// How a call shares out its work (gated_scan_kernels.cuh).
+struct GatedScanSplit {
+  int n_cblk, chunks, runs;  // channel blocks; blocks per column; runs per warp of ranges
+};
+struct GatedScanPlan {
+  GatedScanSplit sp;
+  int nw;  // warps per block
+  bool ranges;
+  long long cols, blocks;
+  // floats of the ranges' maps: a row for each warp and one for each block
+  long long map_floats(int V) const { return ranges ? cols * sp.chunks * (nw + 1) * 64 * V : 0; }
+};
+GatedScanPlan gated_scan_plan(int B, int T, int D, int V);
+bool gated_scan_pairs(const GatedScanArgs& a);
+yuf_status_t gated_scan_dlower(const float* partial, float* dlower, long long rows, int D, cudaStream_t st);
+inline bool gated_aligned(const void* q, size_t bytes) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; }
+inline int gated_elem_size(int dtype) { return dtype == YUF_DTYPE_F32 ? 4 : 2; }
+
 size_t gated_scan_workspace_floats(int B, int T, int D, int dtype, bool backward);
 
 yuf_status_t gated_scan_forward(const GatedScanArgs& a, cudaStream_t st);
