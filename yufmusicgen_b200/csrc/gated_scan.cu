@@ -161,8 +161,8 @@ yuf_status_t gated_scan_step(const void* x, const void* f, const void* g, long l
                              const float* lower, float* state, long long ss, void* y, int dtype, int B, int D,
                              cudaStream_t st) {
   const size_t e = 2 * gated_elem_size(dtype);
-  const bool two = D % 2 == 0 && ((xs | fs | gs | ss) & 1) == 0 && gated_aligned(x, e) && gated_aligned(f, e) && gated_aligned(g, e) &&
-                   gated_aligned(y, e) && gated_aligned(lower, 8) && gated_aligned(state, 8);
+  const bool two = D % 2 == 0 && ((xs | fs | gs | ss) & 1) == 0 && gated_aligned(x, e) && gated_aligned(f, e) &&
+                   gated_aligned(g, e) && gated_aligned(y, e) && gated_aligned(lower, 8) && gated_aligned(state, 8);
 #define STEP(T, V) launch_step<T, V>(x, f, g, xs, fs, gs, lower, state, ss, y, B, D, st)
   switch (dtype) {
     case YUF_DTYPE_F32: return two ? STEP(float, 2) : STEP(float, 1);

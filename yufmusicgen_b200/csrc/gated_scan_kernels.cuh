@@ -323,7 +323,9 @@ YUF_DEVICE void put_row(char* slot, int j, int lane, Fv<V> v) {
   reinterpret_cast<Raw<T, V>*>(slot + j * 128)[lane] = Raw<T, V>::put(v);
 }
 // a lane's word of row j as fp32, for values kept between two passes
-YUF_DEVICE float get_word(const char* slot, int j, int lane) { return reinterpret_cast<const float*>(slot + j * 128)[lane]; }
+YUF_DEVICE float get_word(const char* slot, int j, int lane) {
+  return reinterpret_cast<const float*>(slot + j * 128)[lane];
+}
 YUF_DEVICE void put_word(char* slot, int j, int lane, float v) { reinterpret_cast<float*>(slot + j * 128)[lane] = v; }
 
 // Plain loads of a warp's tokens: one row each, from `q` on; bit j of `lanes`: this lane has one.
@@ -373,37 +375,37 @@ YUF_DEVICE const T* row_ptr(const void* t, long long sb, int b, int c) {
   return static_cast<const T*>(t) + b * sb + c;
 }
 
-// 1 / (1 + e) of token u: every other pair of channels on the FMA pipe (see
-// rcp_1p_newton), which balances the two units.
-template <int V>
+// 1 / (1 + e) of token u.  TURNS: every other pair of channels on the FMA pipe (see
+// rcp_1p_newton), which balances the two units in the whole form.
+template <bool TURNS, int V>
 YUF_DEVICE Fv<V> rcp_turns(Fv<V> e, int u) {
-  if constexpr (V == 2)
+  if constexpr (TURNS && V == 2)
     if (u & 1) return rcp_1p_newton(e);
   return rcp_1p(e);
 }
 // Rates of a group of tokens, and gates of a group.
-template <typename T, int V, int N>
+template <bool TURNS, typename T, int V, int N>
 YUF_DEVICE void group_pairs(const Raw<T, V> (&f)[N], Fv<V> (&s)[N], Fv<V> (&m)[N]) {
 #pragma unroll
   for (int u = 0; u < N; ++u) {
     m[u] = sigmoid_exp(sigmoid_arg(f[u]).get());
-    s[u] = rcp_turns(m[u], u);
+    s[u] = rcp_turns<TURNS>(m[u], u);
     m[u] = mul(m[u], s[u]);
   }
 }
-template <typename T, int V, int N>
+template <bool TURNS, typename T, int V, int N>
 YUF_DEVICE void group_rates(const Columns<T, V>& k, const Raw<T, V> (&f)[N], Fv<V> (&a)[N], Fv<V> (&in)[N]) {
-  group_pairs(f, a, in);
+  group_pairs<TURNS>(f, a, in);
 #pragma unroll
   for (int u = 0; u < N; ++u) {
     a[u] = fma(k.om, a[u], k.lo);
     in[u] = mul(k.om, in[u]);
   }
 }
-template <typename T, int V, int N>
+template <bool TURNS, typename T, int V, int N>
 YUF_DEVICE void group_gates(const Raw<T, V> (&g)[N], Fv<V> (&s)[N]) {
 #pragma unroll
-  for (int u = 0; u < N; ++u) s[u] = rcp_turns(sigmoid_exp(sigmoid_arg(g[u]).get()), u);
+  for (int u = 0; u < N; ++u) s[u] = rcp_turns<TURNS>(sigmoid_exp(sigmoid_arg(g[u]).get()), u);
 }
 
 // ---------------------------------------------------------------------------
@@ -480,7 +482,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         Fv<V> ag[GROUP], in[GROUP];
         take(xv, X, j0);
         take(fv, F, j0);
-        group_rates(k, fv, ag, in);
+        group_rates<true>(k, fv, ag, in);
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
           a[j0 + u] = ag[u];
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         if constexpr (GATE) {
           Raw<T, V> gv[GROUP];
           take(gv, Gt, j0);
-          group_gates(gv, sg);
+          group_gates<true>(gv, sg);
         }
 #pragma unroll
         for (int u = 0; u < GROUP; ++u, yq += p.D) {
@@ -638,7 +640,7 @@ __global__ void __launch_bounds__(32 * NW_MAX)
         Fv<V> a[GROUP], in[GROUP];
         take(xv, X, j0);
         take(fv, F, j0);
-        group_rates(k, fv, a, in);
+        group_rates<false>(k, fv, a, in);
 #pragma unroll
         for (int u = GROUP - 1; u >= 0; --u) {
           H = fma(A, mul(in[u], xv[u].get()), H);
@@ -746,9 +748,9 @@ __global__ void __launch_bounds__(32 * NW_MAX)
         if constexpr (GATE) {
           Raw<T, V> gv[GROUP];
           take(gv, Gt, j0);
-          group_gates(gv, sg);
+          group_gates<false>(gv, sg);
         }
-        group_rates(k, fv, a, in);
+        group_rates<false>(k, fv, a, in);
 #pragma unroll
         for (int u = 0; u < GROUP; ++u, yq += p.D) {
           h = fma(a[u], h, mul(in[u], xv[u].get()));
@@ -941,9 +943,9 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
           if constexpr (GATE) {
             Raw<T, V> gv[N];
             take(gv, Gt, j0);
-            group_gates(gv, sgm);
+            group_gates<!RANGES>(gv, sgm);
           }
-          group_pairs(fv, s, m);
+          group_pairs<!RANGES>(fv, s, m);
 #pragma unroll
           for (int u = 0; u < N; ++u, dgq += p.D) {
             const int j = j0 + u;
@@ -1165,9 +1167,9 @@ __global__ void __launch_bounds__(32 * NW_MAX)
           if constexpr (GATE) {
             Raw<T, V> gv[GROUP];
             take(gv, Gt, j0);
-            group_gates(gv, sg);
+            group_gates<false>(gv, sg);
           }
-          group_rates(k, fv, a, in);
+          group_rates<false>(k, fv, a, in);
 #pragma unroll
           for (int u = 0; u < GROUP; ++u) {
             A = mul(A, a[u]);

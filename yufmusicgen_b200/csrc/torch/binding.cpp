@@ -85,7 +85,8 @@ variable_list once(const char* name, bool recorded, variable_list grads) {
 struct On {
   c10::cuda::CUDAGuard guard;
   void* stream;
-  explicit On(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+  explicit On(const Tensor& t)
+      : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
 };
 
 // ---- gated recurrence -------------------------------------------------------
@@ -102,7 +103,8 @@ struct Inputs {
 
 void check_tokens(const Tensor& x, const Tensor& f, const Tensor& g, const Tensor& lower, int64_t ndim) {
   NEED(x.defined() && f.defined(), TypeError, "gated scan: x and forget must be tensors");
-  NEED(x.dim() == ndim, ValueError, "gated scan: x must have shape ", ndim == 3 ? "[B, T, D]" : "[B, D]", ", got ", x.sizes());
+  NEED(x.dim() == ndim, ValueError, "gated scan: x must have shape ", ndim == 3 ? "[B, T, D]" : "[B, D]", ", got ",
+       x.sizes());
   NEED(x.is_cuda(), ValueError, "gated scan inputs must be on CUDA");
   NEED(dtype_of(x) >= 0, TypeError, "gated scan: x must be float32, bfloat16 or float16, got ", x.scalar_type());
   for (const Tensor* t : {&f, &g})
@@ -145,7 +147,8 @@ std::array<Tensor, 3> scan_forward(const Inputs& in, bool save) {
   const Tensor &x = in.x, &f = in.f, &g = in.g;
   const auto f32 = x.options().dtype(at::kFloat);
   On on(x);
-  Tensor y = at::empty({x.size(0), x.size(1), x.size(2)}, x.options()), last = at::empty({in.rows, x.size(2)}, f32), ckpt;
+  Tensor y = at::empty({x.size(0), x.size(1), x.size(2)}, x.options());
+  Tensor last = at::empty({in.rows, x.size(2)}, f32), ckpt;
   if (save) {
     const int block = yuf_gated_scan_block(in.dtype);
     ckpt = at::empty({x.size(0), (x.size(1) + block - 1) / block, x.size(2)}, f32);
@@ -181,11 +184,10 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
                     ctx->saved_data["rows"].toInt()};
     const Tensor &x = in.x, &f = in.f, &g = in.g;
     On on(x);
-    const Tensor dy = grads[0].defined() ? unit_rows(grads[0]) : at::zeros({x.size(0), x.size(1), x.size(2)}, x.options());
+    const std::array<int64_t, 3> shape{x.size(0), x.size(1), x.size(2)};
+    const Tensor dy = grads[0].defined() ? unit_rows(grads[0]) : at::zeros(shape, x.options());
     const Tensor dlast = dense(grads[1]);
-    const auto like = [&](const Tensor& t) {
-      return t.defined() ? at::empty({x.size(0), x.size(1), x.size(2)}, x.options()) : Tensor();
-    };
+    const auto like = [&](const Tensor& t) { return t.defined() ? at::empty(shape, x.options()) : Tensor(); };
     const Tensor dx = like(x), df = like(f), dg = like(g), work = workspace(in, true);
     Tensor dlower, dstate;
     const int64_t wants = ctx->saved_data["wants"].toInt();
