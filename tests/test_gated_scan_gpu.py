@@ -104,7 +104,8 @@ def infer(v):
 
 
 SHAPES = [(1, 1, 1), (2, 7, 33), (3, 16, 64), (1, 17, 2), (2, 129, 40), (1, 300, 130), (2, 1025, 66), (1, 2048, 640),
-          (5, 64, 31), (300, 3, 10), (1, 1100, 64), (2, 2060, 72), (37, 300, 64), (80, 530, 16), (150, 290, 8)]
+          (5, 64, 31), (300, 3, 10), (1, 1100, 64), (2, 2060, 72), (37, 300, 64), (80, 530, 16), (150, 290, 8),
+          (80, 300, 17)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
@@ -145,6 +146,16 @@ def test_packed_sequences(cu, T, D, dtype):
 def test_packed_without_optional_inputs(gate, state):
     v = make(1, 500, 66, "fp16", gate, False, state, cu=[0, 100, 100, 355, 480], seed=8)
     check(v, *train(v))
+
+
+@pytest.mark.parametrize("D", [2600, 2601])
+def test_packed_wide_rows(D):
+    """So many columns that a block walks a packed row by itself, in several steps."""
+    cu = [0, 100, 100, 430, 590]
+    v = make(1, 600, D, "bf16", cu=cu, seed=D)
+    got, grads = train(v)
+    check(v, got, grads)
+    assert not got[0][:, 590:].any() and not grads["gate"][:, 590:].any()
 
 
 def test_packed_equals_each_sequence_alone_and_shields_it():
