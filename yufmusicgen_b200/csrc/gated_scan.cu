@@ -24,7 +24,7 @@ GatedScanPlan gated_scan_plan(int B, int T, int D, int V) {
   if (p.ranges) {
     // One range for each warp that fits (the slots of 16 warps fill an SM's shared
     // memory); blocks of 4 warps, which leave fewer idle at the end than 8.
-    p.nw = 4;
+    p.nw = GATED_SCAN_RANGE_WARPS;
     const long long runs = (p.cols * T + (long long)L * SMS * 16 - 1) / ((long long)L * SMS * 16);
     p.sp.runs = (int)max(1LL, runs);
     p.sp.chunks = (T + p.nw * L * p.sp.runs - 1) / (p.nw * L * p.sp.runs);

@@ -26,7 +26,8 @@ struct GatedScanArgs {
 
 // tokens between two saved states
 constexpr int GATED_SCAN_BLOCK = 16;
-constexpr int GATED_SCAN_WARPS = 16;  // warps per block, at most
+constexpr int GATED_SCAN_WARPS = 16;       // warps per block, at most
+constexpr int GATED_SCAN_RANGE_WARPS = 4;  // warps per block of ranges
 
 // How a call shares out its work (gated_scan_kernels.cuh).
 struct GatedScanSplit {

@@ -45,6 +45,7 @@ using Plan = GatedScanPlan;
 
 constexpr int L = GATED_SCAN_BLOCK;  // tokens per run; the backward's states are L apart
 constexpr int NW_MAX = GATED_SCAN_WARPS;
+constexpr int RANGE_WARPS = GATED_SCAN_RANGE_WARPS;
 constexpr float CUT = -1.f;          // A of a run that forgets what came before it (A >= 0 otherwise)
 
 __device__ unsigned int g_gated_wait_timeouts;  // of this element type's kernels
@@ -584,7 +585,7 @@ YUF_DEVICE int range_runs(const Split& sp, int t, int T) { return max(0, min(sp.
 // first was read last here and is still in L2.  (The backward's are the other way
 // round by themselves.)
 template <typename T, int V, bool PACKED, bool TMA>
-__global__ void __launch_bounds__(32 * NW_MAX)
+__global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     gated_scan_forward_maps_kernel(const GatedScanArgs p, const __grid_constant__ ScanMaps tm, const Split sp) {
   extern __shared__ __align__(128) char smem[];
   Place at = range_place<false>(sp);
@@ -675,7 +676,7 @@ __global__ void __launch_bounds__(32 * NW_MAX)
 // Each range from its true start state, in one pass.  Two stages of x, f, g; y is
 // stored from registers, so that a stage is loaded again as soon as it is worked off.
 template <typename T, int V, bool GATE, bool PACKED, bool TMA>
-__global__ void __launch_bounds__(32 * NW_MAX)
+__global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     gated_scan_forward_ranges_kernel(const GatedScanArgs p, const __grid_constant__ ScanMaps tm, const Split sp) {
   constexpr int NS = GATE ? 3 : 2;
   extern __shared__ __align__(128) char smem[];
@@ -1090,6 +1091,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         bulk_commit();
       }
     } else if constexpr (TMA) {
+      fence_proxy_async();  // m was put over the slots
       __syncwarp();
       if (lane == 0) issue_xf(i + 2);
     }
@@ -1103,7 +1105,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
 
 // The map of each range, backward: f, dy and g; two stages.  h is not needed.
 template <typename T, int V, bool GATE, bool PACKED, bool TMA>
-__global__ void __launch_bounds__(32 * NW_MAX)
+__global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     gated_scan_backward_maps_kernel(const GatedScanArgs p, const __grid_constant__ ScanMaps tm, const Split sp) {
   constexpr int NS = GATE ? 3 : 2;
   extern __shared__ __align__(128) char smem[];
