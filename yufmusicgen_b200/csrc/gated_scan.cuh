@@ -1,5 +1,5 @@
-// Arguments of the gated recurrence's kernels (gated_scan.cu), filled by the
-// C ABI (ops_capi.cu).
+// Arguments of the gated recurrence's kernels (gated_scan_kernels.cuh) and of dropout
+// (dropout.cu), filled by the C ABI (capi.cu), and what their host sides share.
 #pragma once
 #include "common.cuh"
 
