@@ -127,7 +127,7 @@ def test_optional_inputs(gate, lower, state):
 
 
 PACKED = [([0, 5, 5, 40, 41, 300], 300), ([0, 0, 0, 64], 64), ([0, 0], 7), ([0, 1, 2, 3], 3), ([0, 128, 256], 256),
-          ([0, 127, 129, 129, 129, 1000], 1100), ([0], 5), ([0, 0, 0], 0), ([0, 700], 700), ([0, 200, 200, 257, 260], 270)]
+          ([0, 127, 129, 129, 129, 1000], 1100), ([0], 5), ([0, 0, 0], 0), ([0, 700], 700), ([0, 5000, 5001, 9000], 9000), ([0, 200, 200, 257, 260], 270)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
@@ -145,6 +145,14 @@ def test_packed_sequences(cu, T, D, dtype):
 @pytest.mark.parametrize("gate,state", [(False, False), (True, False), (False, True)])
 def test_packed_without_optional_inputs(gate, state):
     v = make(1, 500, 66, "fp16", gate, False, state, cu=[0, 100, 100, 355, 480], seed=8)
+    check(v, *train(v))
+
+
+@pytest.mark.parametrize("T", [40, 700])
+def test_many_short_and_empty_sequences(T):
+    """Sequences of one token, and dozens of empty ones at one place."""
+    cu = sorted(list(range(0, 30)) + [17] * 40 + [31] * 33 + [33, 38])
+    v = make(1, T, 24, "fp32", cu=cu, seed=T)
     check(v, *train(v))
 
 

@@ -31,6 +31,7 @@
 #include "gated_scan.cuh"
 
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "io_types.cuh"
@@ -221,43 +222,67 @@ struct Run {
   unsigned live;    // inside, and in a sequence
   unsigned first;   // first / last token of its sequence (packed only: the ends of
   unsigned last;    // the row itself are the caller's)
-  int owner;        // lane j + 1: the sequence of token t0 + j
+  int owner;        // lane j + 1: the sequence of token t0 + j, where first or last has bits
+  int from = 0, to = -1;  // a sequence met lately: tokens from .. to - 1
   YUF_DEVICE bool plain() const { return live == (1u << L) - 1 && !(first | last); }
   YUF_DEVICE int owner_of(int j) const { return __shfl_sync(0xffffffffu, owner, j + 1); }
 };
 
-// Sequence of token t: index of the last boundary <= t, -1 before the first,
-// n_seqs at and after the last one.  Any contents of cu give a value in [-1, n_seqs].
-// `hint`: the answer for a token nearby, most often this one's too.
-YUF_DEVICE int find_owner(const int* cu, int n_seqs, int t, int T, int hint) {
-  if (t < 0) return -1;
-  if (t >= T) return n_seqs;
-  if (hint >= 0 && hint < n_seqs) {
-    const int c0 = __ldg(cu + hint), c1 = __ldg(cu + hint + 1);
-    if (c0 <= t && t < c1) return hint;
-  }
-  int lo = 0, hi = n_seqs + 1;  // boundaries before lo are <= t, from hi on > t
+// Boundaries <= t, by the whole warp: each round 32 of them cut the rest to a 32nd.  Any
+// contents of cu give a value in [0, n_seqs + 1].
+YUF_DEVICE int count_boundaries(const int* cu, int n_seqs, int t, int lane) {
+  int lo = 0, hi = n_seqs + 1;  // the answer is in [lo, hi]
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid + 1;
-    else hi = mid;
+    const int step = (hi - lo + 31) / 32, at = min(lo + lane * step, hi);
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && __ldg(cu + min(at, n_seqs)) <= t);
+    const int k = __popc(below);
+    if (k == 0) return lo;
+    hi = min(hi, lo + k * step);
+    lo += (k - 1) * step + 1;
   }
-  return lo - 1;
+  return lo;
 }
 
-// `r` holds the same warp's answer of the step before
-template <bool PACKED>
+// Sequence of lane's token t0 - 1 + lane: the last boundary at or before it, -1 before
+// the first, n_seqs at and after the last one and behind the row.
+YUF_DEVICE int find_owners(const GatedScanArgs& p, int t0, int lane) {
+  const int t = t0 - 1 + lane, o = t0 > 0 ? count_boundaries(p.cu, p.n_seqs, t0 - 1, lane) - 1 : -1;
+  const int bound = lane < p.n_seqs - o ? __ldg(p.cu + o + 1 + lane) : INT_MAX;  // the 32 that follow
+  const int more = __popc(__ballot_sync(0xffffffffu, bound <= t0 + L));
+  int mine = o;
+  if (more < 32) {
+    for (int k = 0; k < more; ++k) mine += __shfl_sync(0xffffffffu, bound, k) <= t;
+  } else {  // empty sequences by the dozen: each lane for itself
+    int lo = o + 1, hi = p.n_seqs + 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(p.cu + mid) <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    mine = lo - 1;
+  }
+  return t < 0 ? -1 : t >= p.T ? p.n_seqs : mine;
+}
+
+// REVERSE: the next run lies before this one.  Within a sequence longer than a run this
+// takes two comparisons.
+template <bool PACKED, bool REVERSE>
 YUF_DEVICE void look(Run& r, const GatedScanArgs& p, int t0, int lane) {
   const int n = max(0, min(L, p.T - t0));
   r.inside = r.live = (1u << n) - 1;
   r.first = r.last = 0;
   if constexpr (PACKED) {
-    if (lane < L + 2) r.owner = find_owner(p.cu, p.n_seqs, t0 - 1 + lane, p.T, r.owner);
+    if (n == 0 || (r.from < t0 && t0 + L < r.to && t0 + L < p.T)) return;
+    r.owner = find_owners(p, t0, lane);
     const int prev = __shfl_up_sync(0xffffffffu, r.owner, 1), next = __shfl_down_sync(0xffffffffu, r.owner, 1);
     const bool mid = lane >= 1 && lane <= L && r.owner >= 0 && r.owner < p.n_seqs;
     r.live = (__ballot_sync(0xffffffffu, mid) >> 1) & r.inside;
     r.first = (__ballot_sync(0xffffffffu, prev != r.owner) >> 1) & r.live;
     r.last = (__ballot_sync(0xffffffffu, next != r.owner) >> 1) & r.live;
+    const int near = __shfl_sync(0xffffffffu, r.owner, REVERSE ? 0 : L + 1);
+    const bool known = near >= 0 && near < p.n_seqs;
+    r.from = known ? __ldg(p.cu + near) : 0;
+    r.to = known ? __ldg(p.cu + near + 1) : -1;
   }
 }
 
@@ -362,13 +387,6 @@ struct Columns {
 #pragma unroll
       for (int i = 0; i < V; ++i) om.v[i] = 1.f - lo.v[i];
     }
-  }
-  // retention a and input share of a token
-  YUF_DEVICE void rates(Raw<T, V> f, Fv<V>& a, Fv<V>& in) const {
-    Fv<V> s, m;
-    sigmoid_pair(sigmoid_arg(f).get(), s, m);
-    a = fma(om, s, lo);
-    in = mul(om, m);
   }
 };
 template <typename T>
@@ -477,11 +495,12 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
       load_rows<T, V>(fr, fp + t0 * p.ft, p.ft, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED>(run, p, t0, lane);
+    look<PACKED, false>(run, p, t0, lane);
     if (TMA && run.inside) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     // this warp's map; a dead token is the identity
     Fv<V> a[L], bx[L], A = splat<V>(1.f), H = splat<V>(0.f);
-    if (run.plain()) {
+    const auto up = [&](auto fast) {  // fast: every token is live, and none first or last
+      constexpr bool F_ = decltype(fast)::value;
 #pragma unroll
       for (int j0 = 0; j0 < L; j0 += GROUP) {
         Raw<T, V> xv[GROUP], fv[GROUP];
@@ -491,30 +510,24 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         group_rates<true>(k, fv, ag, in);
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
-          a[j0 + u] = ag[u];
-          bx[j0 + u] = mul(in[u], xv[u].get());
-          H = fma(ag[u], H, bx[j0 + u]);
-          A = mul(A, ag[u]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        a[j] = splat<V>(1.f);
-        bx[j] = splat<V>(0.f);
-        if (run.live >> j & 1) {
-          Fv<V> in;
-          k.rates(F(j), a[j], in);
-          bx[j] = mul(in, X(j).get());
-          if (run.first >> j & 1) {
+          const int j = j0 + u;
+          a[j] = ag[u];
+          bx[j] = mul(in[u], xv[u].get());
+          if (!F_ && !(run.live >> j & 1)) {
+            a[j] = splat<V>(1.f);
+            bx[j] = splat<V>(0.f);
+          }
+          if (PACKED && !F_ && (run.first >> j & 1)) {
             const Fv<V> h0 = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
             if (p.h0) bx[j] = fma(a[j], h0, bx[j]);
             a[j] = splat<V>(CUT);
           }
-          compose<PACKED>(A, H, a[j], bx[j]);
+          compose<PACKED && !F_>(A, H, a[j], bx[j]);
         }
       }
-    }
+    };
+    if (run.plain()) up(std::true_type{});
+    else if (run.inside) up(std::false_type{});
     if (TMA && lane == 0) {
       bulk_wait_read<0>();  // y of the step before has left the slots that are loaded now
       issue(i + 1);
@@ -522,8 +535,9 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     Fv<V> hw = join<PACKED, V>(joint, at, i, A, H, h);
     if (!run.inside) continue;
     if (p.ckpt && k.act) store_f32<V>(p.ckpt + (k.b * n_ck + t0 / L) * p.D + k.c, hw);
-    T* yq = yp + (long long)t0 * p.D;
-    if (run.plain()) {
+    const auto down = [&](auto fast) {
+      constexpr bool F_ = decltype(fast)::value;
+      T* yq = yp + (long long)t0 * p.D;
 #pragma unroll
       for (int j0 = 0; j0 < L; j0 += GROUP) {
         Fv<V> sg[GROUP];
@@ -534,28 +548,22 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         }
 #pragma unroll
         for (int u = 0; u < GROUP; ++u, yq += p.D) {
-          hw = fma(a[j0 + u], hw, bx[j0 + u]);
+          const int j = j0 + u;
+          hw = apply<PACKED && !F_>(a[j], bx[j], hw);
           Fv<V> y = hw;
           if constexpr (GATE) y = mul(hw, sg[u]);
-          if constexpr (TMA) put_row<T, V>(sx, j0 + u, lane, y);
-          else if (k.act) store_raw<T, V>(yq, y);
+          if (!F_ && !(run.live >> j & 1)) y = splat<V>(0.f);
+          if constexpr (TMA) put_row<T, V>(sx, j, lane, y);
+          else if (F_ ? k.act : lanes >> j & 1) store_raw<T, V>(yq, y);
+          if (PACKED && !F_ && (run.last >> j & 1)) {
+            const int o = run.owner_of(j);
+            if (p.h_last && k.act) store_f32<V>(p.h_last + (long long)o * p.D + k.c, hw);
+          }
         }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < L; ++j, yq += p.D) {
-        hw = apply<PACKED>(a[j], bx[j], hw);
-        Fv<V> y = hw;
-        if constexpr (GATE) y = mul(hw, sigmoid_of(Gt(j).get()));
-        if (!(run.live >> j & 1)) y = splat<V>(0.f);
-        if constexpr (TMA) put_row<T, V>(sx, j, lane, y);
-        else if (lanes >> j & 1) store_raw<T, V>(yq, y);
-        if (PACKED && (run.last >> j & 1)) {
-          const int o = run.owner_of(j);
-          if (p.h_last && k.act) store_f32<V>(p.h_last + (long long)o * p.D + k.c, hw);
-        }
-      }
-    }
+    };
+    if (run.plain()) down(std::true_type{});
+    else down(std::false_type{});
     if constexpr (TMA) {
       fence_proxy_async();
       __syncwarp();
@@ -637,10 +645,10 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       load_rows<T, V>(xr, xp + t0 * p.xt, p.xt, lanes);
       load_rows<T, V>(fr, fp + t0 * p.ft, p.ft, lanes);
     }
-    look<PACKED>(run, p, t0, lane);
+    look<PACKED, true>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
-    if (PACKED && cut) {
-    } else if (run.plain()) {
+    const auto pass = [&](auto fast) {
+      constexpr bool F_ = decltype(fast)::value;
 #pragma unroll
       for (int j0 = L - GROUP; j0 >= 0; j0 -= GROUP) {
         Raw<T, V> xv[GROUP], fv[GROUP];
@@ -650,25 +658,23 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
         group_rates<false>(k, fv, a, in);
 #pragma unroll
         for (int u = GROUP - 1; u >= 0; --u) {
-          H = fma(A, mul(in[u], xv[u].get()), H);
-          A = mul(A, a[u]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = L - 1; j >= 0; --j) {
-        if ((run.live >> j & 1) && !(PACKED && cut)) {
-          Fv<V> a, in;
-          k.rates(F(j), a, in);
-          H = fma(A, mul(in, X(j).get()), H);
-          A = mul(A, a);
-          if (run.first >> j & 1) {
-            if (p.h0) H = fma(A, row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act), H);
-            A = splat<V>(CUT);
-            cut = true;
+          const int j = j0 + u;
+          if (F_ || ((run.live >> j & 1) && !cut)) {
+            H = fma(A, mul(in[u], xv[u].get()), H);
+            A = mul(A, a[u]);
+            if (PACKED && !F_ && (run.first >> j & 1)) {
+              const Fv<V> h0 = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
+              if (p.h0) H = fma(A, h0, H);
+              A = splat<V>(CUT);
+              cut = true;
+            }
           }
         }
       }
+    };
+    if (!cut) {
+      if (run.plain()) pass(std::true_type{});
+      else pass(std::false_type{});
     }
     if constexpr (TMA) {
       __syncwarp();
@@ -743,11 +749,12 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       load_rows<T, V>(fr, fp + t0 * p.ft, p.ft, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED>(run, p, t0, lane);
+    look<PACKED, false>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     if (p.ckpt && k.act) store_f32<V>(p.ckpt + (k.b * n_ck + t0 / L) * p.D + k.c, h);
-    T* yq = yp + (long long)t0 * p.D;
-    if (run.plain()) {
+    const auto pass = [&](auto fast) {
+      constexpr bool F_ = decltype(fast)::value;
+      T* yq = yp + (long long)t0 * p.D;
 #pragma unroll
       for (int j0 = 0; j0 < L; j0 += GROUP) {
         Raw<T, V> xv[GROUP], fv[GROUP];
@@ -762,31 +769,24 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
         group_rates<false>(k, fv, a, in);
 #pragma unroll
         for (int u = 0; u < GROUP; ++u, yq += p.D) {
-          h = fma(a[u], h, mul(in[u], xv[u].get()));
-          Fv<V> y = h;
-          if constexpr (GATE) y = mul(h, sg[u]);
-          if (k.act) store_raw<T, V>(yq, y);
+          const int j = j0 + u;
+          Fv<V> y = splat<V>(0.f);
+          if (F_ || (run.live >> j & 1)) {
+            if (PACKED && !F_ && (run.first >> j & 1)) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
+            h = fma(a[u], h, mul(in[u], xv[u].get()));
+            y = h;
+            if constexpr (GATE) y = mul(h, sg[u]);
+          }
+          if (F_ ? k.act : lanes >> j & 1) store_raw<T, V>(yq, y);
+          if (PACKED && !F_ && (run.last >> j & 1)) {
+            const int o = run.owner_of(j);
+            if (p.h_last && k.act) store_f32<V>(p.h_last + (long long)o * p.D + k.c, h);
+          }
         }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < L; ++j, yq += p.D) {
-        Fv<V> y = splat<V>(0.f);
-        if (run.live >> j & 1) {
-          Fv<V> a, in;
-          k.rates(F(j), a, in);
-          if (run.first >> j & 1) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
-          h = fma(a, h, mul(in, X(j).get()));
-          y = h;
-          if constexpr (GATE) y = mul(h, sigmoid_of(Gt(j).get()));
-        }
-        if (lanes >> j & 1) store_raw<T, V>(yq, y);
-        if (PACKED && (run.last >> j & 1)) {
-          const int o = run.owner_of(j);
-          if (p.h_last && k.act) store_f32<V>(p.h_last + (long long)o * p.D + k.c, h);
-        }
-      }
-    }
+    };
+    if (run.plain()) pass(std::true_type{});
+    else pass(std::false_type{});
     if constexpr (TMA) {
       __syncwarp();
       if (lane == 0) issue(i + 2);
@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
       load_rows<T, V>(dr, dyp + t0 * p.yt, p.yt, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED>(run, p, t0, lane);
+    look<PACKED, true>(run, p, t0, lane);
     const bool plain = run.plain();
     if (TMA && run.inside) {
       const int miss = i - seen;  // 0, or 1 where the first step had no tokens
@@ -942,87 +942,58 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     const auto up = [&](auto fast) {  // fast: every token is live, and none first or last
       constexpr bool F_ = decltype(fast)::value;
       T* dgq = GATE ? static_cast<T*>(p.dg) + row0 : nullptr;
-      if constexpr (F_) {
-        constexpr int N = 4;  // as many as the registers hold beside e and q
+      constexpr int N = 4;  // as many as the registers hold beside e and q
 #pragma unroll
-        for (int j0 = 0; j0 < L; j0 += N) {
-          Raw<T, V> xv[N], fv[N], dv[N];
-          Fv<V> s[N], m[N], sgm[N];
-          take(xv, X, j0);
-          take(fv, F, j0);
-          take(dv, Dy, j0);
-          if constexpr (GATE) {
-            Raw<T, V> gv[N];
-            take(gv, Gt, j0);
-            group_gates<!RANGES>(gv, sgm);
+      for (int j0 = 0; j0 < L; j0 += N) {
+        Raw<T, V> xv[N], fv[N], dv[N];
+        Fv<V> s[N], m[N], sgm[N];
+        take(xv, X, j0);
+        take(fv, F, j0);
+        take(dv, Dy, j0);
+        if constexpr (GATE) {
+          Raw<T, V> gv[N];
+          take(gv, Gt, j0);
+          group_gates<!RANGES>(gv, sgm);
+        }
+        group_pairs<!RANGES>(fv, s, m);
+#pragma unroll
+        for (int u = 0; u < N; ++u, dgq += p.D) {
+          const int j = j0 + u;
+          const bool live = F_ || (run.live >> j & 1);
+          const Fv<V> xu = xv[u].get(), a = fma(k.om, s[u], k.lo);
+          if constexpr (TMA) {
+            put_word(sx, j, lane, m[u].v[0]);
+            if constexpr (V == 2) put_word(sf, j, lane, m[u].v[V - 1]);
           }
-          group_pairs<!RANGES>(fv, s, m);
-#pragma unroll
-          for (int u = 0; u < N; ++u, dgq += p.D) {
-            const int j = j0 + u;
-            const Fv<V> xu = xv[u].get(), a = fma(k.om, s[u], k.lo);
-            if constexpr (TMA) {
-              put_word(sx, j, lane, m[u].v[0]);
-              if constexpr (V == 2) put_word(sf, j, lane, m[u].v[V - 1]);
-            }
+          if (PACKED && !F_ && (run.first >> j & 1)) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
+          Fv<V> dg = splat<V>(0.f);
+          e[j] = q[j] = splat<V>(0.f);
+          if (live) {
             e[j] = fma(xu, splat<V>(-1.f), h);
             h = fma(a, h, mul(mul(k.om, m[u]), xu));
             q[j] = dv[u].get();
             if constexpr (GATE) {
               q[j] = mul(q[j], sgm[u]);
-              const Fv<V> dg = mul(mul(q[j], h), fma(sgm[u], splat<V>(-1.f), splat<V>(1.f)));
-              if constexpr (OUT_SLOT) put_row<T, V>(sg, j, lane, dg);
-              else if (k.act) store_raw<T, V>(dgq, dg);
-            }
-            if constexpr (!RANGES) {
-              A = mul(A, a);
-              H = fma(A, q[j], H);
+              dg = mul(mul(q[j], h), fma(sgm[u], splat<V>(-1.f), splat<V>(1.f)));
             }
           }
-        }
-        return;
-      }
-#pragma unroll
-      for (int j = 0; j < L; ++j, dgq += p.D) {
-        e[j] = q[j] = splat<V>(0.f);
-        if (run.live >> j & 1) {
-          Fv<V> s, m;
-          if (PACKED && (run.first >> j & 1)) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
-          const Fv<V> xv = X(j).get();
-          e[j] = fma(xv, splat<V>(-1.f), h);
-          sigmoid_pair(sigmoid_arg(F(j)).get(), s, m);
-          if constexpr (TMA) {
-            put_word(sx, j, lane, m.v[0]);
-            if constexpr (V == 2) put_word(sf, j, lane, m.v[V - 1]);
-          }
-          const Fv<V> a = fma(k.om, s, k.lo);
-          h = fma(a, h, mul(mul(k.om, m), xv));
-          q[j] = Dy(j).get();
-          if constexpr (GATE) {
-            const Fv<V> sgm = sigmoid_of(Gt(j).get());
-            q[j] = mul(q[j], sgm);
-            const Fv<V> dg = mul(mul(q[j], h), fma(sgm, splat<V>(-1.f), splat<V>(1.f)));
-            if constexpr (OUT_SLOT) put_row<T, V>(sg, j, lane, dg);
-            else if (k.act) store_raw<T, V>(dgq, dg);
-          }
-          if (!RANGES && (!PACKED || !cut)) {
+          if constexpr (OUT_SLOT && GATE) put_row<T, V>(sg, j, lane, dg);
+          else if (GATE && (F_ ? k.act : lanes >> j & 1)) store_raw<T, V>(dgq, dg);
+          if (!RANGES && live && !(PACKED && !F_ && cut)) {
             A = mul(A, a);
             H = fma(A, q[j], H);
-            if (PACKED && (run.last >> j & 1)) {
+            if (PACKED && !F_ && (run.last >> j & 1)) {
               const Fv<V> end = row_of<V>(p.dh_last, run.owner_of(j), p.D, k.c, k.act);
               if (p.dh_last) H = fma(A, end, H);
               A = splat<V>(CUT);
               cut = true;
             }
           }
-        } else if (GATE && (run.inside >> j & 1)) {
-          if constexpr (OUT_SLOT) put_row<T, V>(sg, j, lane, splat<V>(0.f));
-          else if (k.act) store_raw<T, V>(dgq, splat<V>(0.f));
         }
       }
     };
     if (plain) up(std::true_type{});
-    else up(std::false_type{});
+    else if (run.inside) up(std::false_type{});  // a step without tokens leaves its slots alone
     if (TMA && run.inside) {
       if constexpr (GATE && OUT_SLOT) fence_proxy_async();
       __syncwarp();
@@ -1166,53 +1137,41 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       load_rows<T, V>(dr, dyp + t0 * p.yt, p.yt, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED>(run, p, t0, lane);
+    look<PACKED, false>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     const auto pass = [&](auto fast) {
       constexpr bool F_ = decltype(fast)::value;
-      if constexpr (F_) {
 #pragma unroll
-        for (int j0 = 0; j0 < L; j0 += GROUP) {
-          Raw<T, V> fv[GROUP], dv[GROUP];
-          Fv<V> a[GROUP], in[GROUP], sg[GROUP];
-          take(fv, F, j0);
-          take(dv, Dy, j0);
-          if constexpr (GATE) {
-            Raw<T, V> gv[GROUP];
-            take(gv, Gt, j0);
-            group_gates<false>(gv, sg);
-          }
-          group_rates<false>(k, fv, a, in);
+      for (int j0 = 0; j0 < L; j0 += GROUP) {
+        Raw<T, V> fv[GROUP], dv[GROUP];
+        Fv<V> a[GROUP], in[GROUP], sg[GROUP];
+        take(fv, F, j0);
+        take(dv, Dy, j0);
+        if constexpr (GATE) {
+          Raw<T, V> gv[GROUP];
+          take(gv, Gt, j0);
+          group_gates<false>(gv, sg);
+        }
+        group_rates<false>(k, fv, a, in);
 #pragma unroll
-          for (int u = 0; u < GROUP; ++u) {
+        for (int u = 0; u < GROUP; ++u) {
+          const int j = j0 + u;
+          if (F_ || ((run.live >> j & 1) && !cut)) {
             A = mul(A, a[u]);
             H = fma(A, GATE ? mul(dv[u].get(), sg[u]) : dv[u].get(), H);
-          }
-        }
-        return;
-      }
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        if ((run.live >> j & 1) && !(PACKED && cut)) {
-          Fv<V> a, in, q = Dy(j).get();
-          k.rates(F(j), a, in);
-          if constexpr (GATE) q = mul(q, sigmoid_of(Gt(j).get()));
-          A = mul(A, a);
-          H = fma(A, q, H);
-          if (PACKED && (run.last >> j & 1)) {
-            const Fv<V> end = row_of<V>(p.dh_last, run.owner_of(j), p.D, k.c, k.act);
-            if (p.dh_last) H = fma(A, end, H);
-            A = splat<V>(CUT);
-            cut = true;
+            if (PACKED && !F_ && (run.last >> j & 1)) {
+              const Fv<V> end = row_of<V>(p.dh_last, run.owner_of(j), p.D, k.c, k.act);
+              if (p.dh_last) H = fma(A, end, H);
+              A = splat<V>(CUT);
+              cut = true;
+            }
           }
         }
       }
     };
-    if (PACKED && cut) {
-    } else if (run.plain()) {
-      pass(std::true_type{});
-    } else {
-      pass(std::false_type{});
+    if (!cut) {
+      if (run.plain()) pass(std::true_type{});
+      else pass(std::false_type{});
     }
     if constexpr (TMA) {
       __syncwarp();
