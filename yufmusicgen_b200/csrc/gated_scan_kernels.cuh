@@ -223,7 +223,9 @@ struct Run {
   unsigned first;   // first / last token of its sequence (packed only: the ends of
   unsigned last;    // the row itself are the caller's)
   int owner;        // lane j + 1: the sequence of token t0 + j, where first or last has bits
-  int from = 0, to = -1;  // a sequence met lately: tokens from .. to - 1
+  // Known of cu_seqlens: lane i holds boundary base + i (packed only), and from .. to - 1
+  // are the tokens of a sequence met lately.
+  int base = -1, bound = INT_MAX, from = 0, to = -1;
   YUF_DEVICE bool plain() const { return live == (1u << L) - 1 && !(first | last); }
   YUF_DEVICE int owner_of(int j) const { return __shfl_sync(0xffffffffu, owner, j + 1); }
 };
@@ -243,23 +245,43 @@ YUF_DEVICE int count_boundaries(const int* cu, int n_seqs, int t, int lane) {
   return lo;
 }
 
+// Whether lanes' boundaries say all about tokens t0 - 1 .. t0 + L.
+YUF_DEVICE bool window_covers(const Run& r, int n_seqs, int t0) {
+  const int first = __shfl_sync(0xffffffffu, r.bound, 0), last = __shfl_sync(0xffffffffu, r.bound, 31);
+  return r.base >= 0 && (r.base == 0 || first < t0) && (r.base + 32 > n_seqs || last > t0 + L);
+}
+
 // Sequence of lane's token t0 - 1 + lane: the last boundary at or before it, -1 before
-// the first, n_seqs at and after the last one and behind the row.
-YUF_DEVICE int find_owners(const GatedScanArgs& p, int t0, int lane) {
-  const int t = t0 - 1 + lane, o = t0 > 0 ? count_boundaries(p.cu, p.n_seqs, t0 - 1, lane) - 1 : -1;
-  const int bound = lane < p.n_seqs - o ? __ldg(p.cu + o + 1 + lane) : INT_MAX;  // the 32 that follow
-  const int more = __popc(__ballot_sync(0xffffffffu, bound <= t0 + L));
-  int mine = o;
-  if (more < 32) {
-    for (int k = 0; k < more; ++k) mine += __shfl_sync(0xffffffffu, bound, k) <= t;
+// the first, n_seqs at and after the last one and behind the row.  With up to 31
+// sequences the boundaries are read once.
+template <bool REVERSE>
+YUF_DEVICE int find_owners(Run& r, const GatedScanArgs& p, int t0, int lane) {
+  const int t = t0 - 1 + lane;
+  bool covers = window_covers(r, p.n_seqs, t0);
+  if (!covers) {
+    r.base = 0;
+    if (p.n_seqs >= 32) {  // most of the window on the side where the next run lies
+      const int before = t0 > 0 ? count_boundaries(p.cu, p.n_seqs, t0 - 1, lane) : 0;
+      r.base = max(0, REVERSE ? before - 24 : before - 1);
+    }
+    r.bound = lane <= p.n_seqs - r.base ? __ldg(p.cu + r.base + lane) : INT_MAX;
+    covers = window_covers(r, p.n_seqs, t0);
+  }
+  int mine;
+  if (covers) {
+    const int c0 = __popc(__ballot_sync(0xffffffffu, r.bound < t0)),
+              c1 = __popc(__ballot_sync(0xffffffffu, r.bound <= t0 + L));
+    mine = r.base - 1 + c0;
+    for (int k = c0; k < c1; ++k) mine += __shfl_sync(0xffffffffu, r.bound, k) <= t;
   } else {  // empty sequences by the dozen: each lane for itself
-    int lo = o + 1, hi = p.n_seqs + 1;
+    int lo = 0, hi = p.n_seqs + 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (__ldg(p.cu + mid) <= t) lo = mid + 1;
       else hi = mid;
     }
     mine = lo - 1;
+    r.base = -1;
   }
   return t < 0 ? -1 : t >= p.T ? p.n_seqs : mine;
 }
@@ -273,16 +295,17 @@ YUF_DEVICE void look(Run& r, const GatedScanArgs& p, int t0, int lane) {
   r.first = r.last = 0;
   if constexpr (PACKED) {
     if (n == 0 || (r.from < t0 && t0 + L < r.to && t0 + L < p.T)) return;
-    r.owner = find_owners(p, t0, lane);
+    r.owner = find_owners<REVERSE>(r, p, t0, lane);
     const int prev = __shfl_up_sync(0xffffffffu, r.owner, 1), next = __shfl_down_sync(0xffffffffu, r.owner, 1);
     const bool mid = lane >= 1 && lane <= L && r.owner >= 0 && r.owner < p.n_seqs;
     r.live = (__ballot_sync(0xffffffffu, mid) >> 1) & r.inside;
     r.first = (__ballot_sync(0xffffffffu, prev != r.owner) >> 1) & r.live;
     r.last = (__ballot_sync(0xffffffffu, next != r.owner) >> 1) & r.live;
-    const int near = __shfl_sync(0xffffffffu, r.owner, REVERSE ? 0 : L + 1);
-    const bool known = near >= 0 && near < p.n_seqs;
-    r.from = known ? __ldg(p.cu + near) : 0;
-    r.to = known ? __ldg(p.cu + near + 1) : -1;
+    const int at = __shfl_sync(0xffffffffu, r.owner, REVERSE ? 0 : L + 1) - r.base;
+    const bool known = r.base >= 0 && at >= 0 && at < 31 && r.base + at < p.n_seqs;
+    const int from = __shfl_sync(0xffffffffu, r.bound, at & 31), to = __shfl_sync(0xffffffffu, r.bound, (at + 1) & 31);
+    r.from = known ? from : 0;
+    r.to = known ? to : -1;
   }
 }
 
@@ -474,6 +497,8 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     }
     __syncwarp();
   }
+  Run run{};
+  look<PACKED, false>(run, p, w * L, lane);  // while the first loads are under way
   Fv<V> h = splat<V>(0.f);
   if constexpr (PACKED) {
     if (p.h_last && k.act) empty_sequences<V>(p, p.h0, p.h_last, k.c, w, nw);
@@ -481,8 +506,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     h = row_of<V>(p.h0, k.b, p.D, k.c, k.act);
   }
 
-  Run run{};
-  for (int i = 0; i < steps; ++i) {
+    for (int i = 0; i < steps; ++i) {
     const int t0 = i * stride + w * L;
     char* const sx = mine + (i & 1) * NS * SLOT;
     Raw<T, V> xr[TMA ? 1 : L], fr[TMA ? 1 : L], gr[TMA ? 1 : L];
@@ -495,7 +519,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
       load_rows<T, V>(fr, fp + t0 * p.ft, p.ft, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED, false>(run, p, t0, lane);
+    if (i > 0) look<PACKED, false>(run, p, t0, lane);
     if (TMA && run.inside) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     // this warp's map; a dead token is the identity
     Fv<V> a[L], bx[L], A = splat<V>(1.f), H = splat<V>(0.f);
@@ -632,6 +656,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     __syncwarp();
   }
   Run run{};
+  look<PACKED, true>(run, p, t_of(0), lane);  // while the first loads are under way
   Fv<V> A = splat<V>(1.f), H = splat<V>(0.f);
   bool cut = false;  // before a first token nothing reaches the range's end any more
   for (int i = 0; i < n; ++i) {
@@ -645,7 +670,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       load_rows<T, V>(xr, xp + t0 * p.xt, p.xt, lanes);
       load_rows<T, V>(fr, fp + t0 * p.ft, p.ft, lanes);
     }
-    look<PACKED, true>(run, p, t0, lane);
+    if (i > 0) look<PACKED, true>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     const auto pass = [&](auto fast) {
       constexpr bool F_ = decltype(fast)::value;
@@ -726,6 +751,8 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     }
     __syncwarp();
   }
+  Run run{};
+  look<PACKED, false>(run, p, r0, lane);  // while the first loads are under way
   Fv<V> h = splat<V>(0.f);
   if constexpr (PACKED) {
     if (p.h_last && k.act) empty_sequences<V>(p, p.h0, p.h_last, k.c, at.chunk * nw + w, sp.chunks * nw);
@@ -735,8 +762,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
   pdl_wait();
   h = take_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), h);
 
-  Run run{};
-  for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < n; ++i) {
     const int t0 = r0 + i * L;
     char* const sx = mine + (i & 1) * NS * SLOT;
     Raw<T, V> xr[TMA ? 1 : L], fr[TMA ? 1 : L], gr[TMA ? 1 : L];
@@ -749,7 +775,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       load_rows<T, V>(fr, fp + t0 * p.ft, p.ft, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED, false>(run, p, t0, lane);
+    if (i > 0) look<PACKED, false>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     if (p.ckpt && k.act) store_f32<V>(p.ckpt + (k.b * n_ck + t0 / L) * p.D + k.c, h);
     const auto pass = [&](auto fast) {
@@ -884,6 +910,8 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     }
     __syncwarp();
   }
+  Run run{};
+  look<PACKED, true>(run, p, t_of(0), lane);  // while the first loads are under way
   Fv<V> G = splat<V>(0.f), dlo = splat<V>(0.f);
   if constexpr (PACKED) {
     if (p.dh0 && k.act) empty_sequences<V>(p, p.dh_last, p.dh0, k.c, at.chunk * nw + w, sp.chunks * nw);
@@ -895,8 +923,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     G = take_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), G);
   }
 
-  Run run{};
-  int seen = 0;  // steps with tokens
+    int seen = 0;  // steps with tokens
   for (int i = 0; i < steps; ++i) {
     const int t0 = t_of(i);
     char* const sx = mine + (i & 1) * 2 * SLOT;
@@ -925,7 +952,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
       load_rows<T, V>(dr, dyp + t0 * p.yt, p.yt, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED, true>(run, p, t0, lane);
+    if (i > 0) look<PACKED, true>(run, p, t0, lane);
     const bool plain = run.plain();
     if (TMA && run.inside) {
       const int miss = i - seen;  // 0, or 1 where the first step had no tokens
@@ -1122,6 +1149,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     __syncwarp();
   }
   Run run{};
+  look<PACKED, false>(run, p, r0, lane);  // while the first loads are under way
   Fv<V> A = splat<V>(1.f), H = splat<V>(0.f);
   bool cut = false;  // behind a last token nothing reaches the range's start any more
   for (int i = 0; i < n; ++i) {
@@ -1137,7 +1165,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       load_rows<T, V>(dr, dyp + t0 * p.yt, p.yt, lanes);
       if constexpr (GATE) load_rows<T, V>(gr, gp + t0 * p.gt, p.gt, lanes);
     }
-    look<PACKED, false>(run, p, t0, lane);
+    if (i > 0) look<PACKED, false>(run, p, t0, lane);
     if constexpr (TMA) check_wait(at, mbar_wait(&full[i & 1], (i >> 1) & 1, at.limit));
     const auto pass = [&](auto fast) {
       constexpr bool F_ = decltype(fast)::value;
