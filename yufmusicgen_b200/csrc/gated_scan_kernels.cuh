@@ -969,52 +969,68 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     const auto up = [&](auto fast) {  // fast: every token is live, and none first or last
       constexpr bool F_ = decltype(fast)::value;
       T* dgq = GATE ? static_cast<T*>(p.dg) + row0 : nullptr;
-      constexpr int N = 4;  // as many as the registers hold beside e and q
-#pragma unroll
-      for (int j0 = 0; j0 < L; j0 += N) {
-        Raw<T, V> xv[N], fv[N], dv[N];
-        Fv<V> s[N], m[N], sgm[N];
-        take(xv, X, j0);
-        take(fv, F, j0);
-        take(dv, Dy, j0);
-        if constexpr (GATE) {
-          Raw<T, V> gv[N];
-          take(gv, Gt, j0);
-          group_gates<!RANGES>(gv, sgm);
+      const auto token = [&](int j, Fv<V> xv, Fv<V> s, Fv<V> m, Fv<V> dyv, Fv<V> sgm, T* dg_at) {
+        const Fv<V> a = fma(k.om, s, k.lo);
+        if constexpr (TMA) {
+          put_word(sx, j, lane, m.v[0]);
+          if constexpr (V == 2) put_word(sf, j, lane, m.v[V - 1]);
         }
-        group_pairs<!RANGES>(fv, s, m);
-#pragma unroll
-        for (int u = 0; u < N; ++u, dgq += p.D) {
-          const int j = j0 + u;
-          const bool live = F_ || (run.live >> j & 1);
-          const Fv<V> xu = xv[u].get(), a = fma(k.om, s[u], k.lo);
-          if constexpr (TMA) {
-            put_word(sx, j, lane, m[u].v[0]);
-            if constexpr (V == 2) put_word(sf, j, lane, m[u].v[V - 1]);
-          }
-          if (PACKED && !F_ && (run.first >> j & 1)) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
-          Fv<V> dg = splat<V>(0.f);
+        if (!F_ && !(run.live >> j & 1)) {
           e[j] = q[j] = splat<V>(0.f);
-          if (live) {
-            e[j] = fma(xu, splat<V>(-1.f), h);
-            h = fma(a, h, mul(mul(k.om, m[u]), xu));
-            q[j] = dv[u].get();
-            if constexpr (GATE) {
-              q[j] = mul(q[j], sgm[u]);
-              dg = mul(mul(q[j], h), fma(sgm[u], splat<V>(-1.f), splat<V>(1.f)));
-            }
+          if constexpr (GATE && OUT_SLOT) put_row<T, V>(sg, j, lane, e[j]);
+          else if (GATE && (lanes >> j & 1)) store_raw<T, V>(dg_at, e[j]);
+          return;
+        }
+        if (PACKED && !F_ && (run.first >> j & 1)) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
+        e[j] = fma(xv, splat<V>(-1.f), h);
+        h = fma(a, h, mul(mul(k.om, m), xv));
+        q[j] = dyv;
+        if constexpr (GATE) {
+          q[j] = mul(q[j], sgm);
+          const Fv<V> dg = mul(mul(q[j], h), fma(sgm, splat<V>(-1.f), splat<V>(1.f)));
+          if constexpr (OUT_SLOT) put_row<T, V>(sg, j, lane, dg);
+          else if (k.act) store_raw<T, V>(dg_at, dg);
+        }
+        if (!RANGES && !(PACKED && !F_ && cut)) {
+          A = mul(A, a);
+          H = fma(A, q[j], H);
+          if (PACKED && !F_ && (run.last >> j & 1)) {
+            const Fv<V> end = row_of<V>(p.dh_last, run.owner_of(j), p.D, k.c, k.act);
+            if (p.dh_last) H = fma(A, end, H);
+            A = splat<V>(CUT);
+            cut = true;
           }
-          if constexpr (OUT_SLOT && GATE) put_row<T, V>(sg, j, lane, dg);
-          else if (GATE && (F_ ? k.act : lanes >> j & 1)) store_raw<T, V>(dgq, dg);
-          if (!RANGES && live && !(PACKED && !F_ && cut)) {
-            A = mul(A, a);
-            H = fma(A, q[j], H);
-            if (PACKED && !F_ && (run.last >> j & 1)) {
-              const Fv<V> end = row_of<V>(p.dh_last, run.owner_of(j), p.D, k.c, k.act);
-              if (p.dh_last) H = fma(A, end, H);
-              A = splat<V>(CUT);
-              cut = true;
-            }
+        }
+      };
+      if constexpr (F_ || (PACKED && (TMA || V == 1))) {
+        constexpr int N = 4;  // as many as the registers hold beside e and q
+#pragma unroll
+        for (int j0 = 0; j0 < L; j0 += N) {
+          Raw<T, V> xv[N], fv[N], dv[N];
+          Fv<V> s[N], m[N], sgm[N];
+          take(xv, X, j0);
+          take(fv, F, j0);
+          take(dv, Dy, j0);
+          if constexpr (GATE) {
+            Raw<T, V> gv[N];
+            take(gv, Gt, j0);
+            group_gates<!RANGES>(gv, sgm);
+          }
+          group_pairs<!RANGES>(fv, s, m);
+#pragma unroll
+          for (int u = 0; u < N; ++u, dgq += p.D) token(j0 + u, xv[u].get(), s[u], m[u], dv[u].get(), sgm[u], dgq);
+        }
+      } else {  // a row's end; pairs without slots, whose raw rows leave no registers for a group
+#pragma unroll
+        for (int j = 0; j < L; ++j, dgq += p.D) {
+          e[j] = q[j] = splat<V>(0.f);
+          if (run.live >> j & 1) {
+            Fv<V> s, m, sgm;
+            sigmoid_pair(sigmoid_arg(F(j)).get(), s, m);
+            if constexpr (GATE) sgm = sigmoid_of(Gt(j).get());
+            token(j, X(j).get(), s, m, Dy(j).get(), sgm, dgq);
+          } else if (GATE && (lanes >> j & 1)) {
+            store_raw<T, V>(dgq, splat<V>(0.f));
           }
         }
       }
