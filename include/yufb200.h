@@ -195,9 +195,10 @@ enum { YUF_DTYPE_F32 = 0, YUF_DTYPE_BF16 = 1, YUF_DTYPE_F16 = 2 };
  *   h0              : [B, D] fp32 initial state ([n_seqs, D] when packed), NULL = 0
  *   cu_seqlens      : NULL, or device [n_seqs + 1], non-decreasing: B must be 1 and
  *                     rows cu[s] .. cu[s+1] - 1 are sequence s, each with its own
- *                     state; a sequence may be empty.  Rows in no sequence are not
- *                     read and get y = 0.  The contents are not checked (wrong ones
- *                     give wrong values, never an access out of bounds).
+ *                     state; a sequence may be empty.  Rows in no sequence play no
+ *                     part, whatever they hold, and get y = 0.  The contents are not
+ *                     checked (wrong ones give wrong values, never an access out of
+ *                     bounds).
  *   y               : [B, T, D] of `dtype`, contiguous
  *   h_last          : [B, D] ([n_seqs, D]) fp32 final state, or NULL.  An empty
  *                     sequence's is its h0.  Must not overlap h0.
@@ -206,7 +207,7 @@ enum { YUF_DTYPE_F32 = 0, YUF_DTYPE_BF16 = 1, YUF_DTYPE_F16 = 2 };
  *   workspace       : yuf_gated_scan_workspace_bytes bytes of device memory, 16-byte
  *                     aligned (NULL where that is 0); its contents before the call do
  *                     not matter, and calls that may run at once need one each
- * Outputs must not overlap inputs.  Any T <= 2^30, any D. */
+ * Outputs must not overlap inputs.  T <= 2^30; any D; B ceil(D / 32) <= 2^26. */
 yuf_status_t yuf_gated_scan_forward(const void* x, const void* forget, const void* gate,
                                     const int64_t* strides, const float* lower, const float* h0,
                                     const int32_t* cu_seqlens, int n_seqs, void* y, float* h_last,

@@ -659,7 +659,8 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
   look<PACKED, true>(run, p, t_of(0), lane);  // while the first loads are under way
   Fv<V> A = splat<V>(1.f), H = splat<V>(0.f);
   bool cut = false;  // before a first token nothing reaches the range's end any more
-  for (int i = 0; i < n; ++i) {
+  int upto = n;  // behind a cut only what is under way is waited for
+  for (int i = 0; i < upto; ++i) {
     const int t0 = t_of(i);
     char* const sx = mine + (i & 1) * 2 * SLOT;
     Raw<T, V> xr[TMA ? 1 : L], fr[TMA ? 1 : L];
@@ -701,9 +702,10 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       if (run.plain()) pass(std::true_type{});
       else pass(std::false_type{});
     }
+    if (PACKED && cut) upto = min(upto, TMA ? i + 2 : i + 1);
     if constexpr (TMA) {
       __syncwarp();
-      if (lane == 0) issue(i + 2);
+      if (lane == 0 && i + 2 < upto) issue(i + 2);
     }
   }
   leave_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), A, H);
@@ -1168,7 +1170,8 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
   look<PACKED, false>(run, p, r0, lane);  // while the first loads are under way
   Fv<V> A = splat<V>(1.f), H = splat<V>(0.f);
   bool cut = false;  // behind a last token nothing reaches the range's start any more
-  for (int i = 0; i < n; ++i) {
+  int upto = n;  // behind a cut only what is under way is waited for
+  for (int i = 0; i < upto; ++i) {
     const int t0 = r0 + i * L;
     char* const sf = mine + (i & 1) * NS * SLOT;
     Raw<T, V> fr[TMA ? 1 : L], dr[TMA ? 1 : L], gr[TMA ? 1 : L];
@@ -1217,9 +1220,10 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
       if (run.plain()) pass(std::true_type{});
       else pass(std::false_type{});
     }
+    if (PACKED && cut) upto = min(upto, TMA ? i + 2 : i + 1);
     if constexpr (TMA) {
       __syncwarp();
-      if (lane == 0) issue(i + 2);
+      if (lane == 0 && i + 2 < upto) issue(i + 2);
     }
   }
   leave_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), A, H);
