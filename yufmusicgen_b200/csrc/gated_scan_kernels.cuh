@@ -1329,7 +1329,8 @@ yuf_status_t backward_with(const GatedScanArgs& a, const ScanMaps& m, cudaStream
   const int j = p.ranges ? maps_bytes(V, p.nw) : join_bytes(V, p.nw);
   const int s = (TMA ? p.nw * (bwd_slots(GATE) * SLOT + 32) : 0) + j;
   GatedScanArgs b = a;
-  if (a.dlower) b.partial = a.work + p.map_floats(V);
+  const long long shares = (long long)a.B * p.sp.chunks;  // of dlower
+  if (a.dlower) b.partial = shares == 1 ? a.dlower : a.work + p.map_floats(V);
   yuf_status_t rc;
   if (!p.ranges) {
     rc = launch<gated_scan_backward_kernel<T, V, GATE, PACKED, TMA, false>>("gated_scan_backward_kernel", b, m, p.sp, p,
@@ -1342,8 +1343,8 @@ yuf_status_t backward_with(const GatedScanArgs& a, const ScanMaps& m, cudaStream
       rc = launch<gated_scan_backward_kernel<T, V, GATE, PACKED, TMA, true>>("gated_scan_backward_kernel (ranges)", b, m,
                                                                              p.sp, p, s, true, st);
   }
-  if (rc != YUF_OK || !a.dlower) return rc;
-  return gated_scan_dlower(b.partial, a.dlower, (long long)a.B * p.sp.chunks, a.D, st);
+  if (rc != YUF_OK || !a.dlower || shares == 1) return rc;
+  return gated_scan_dlower(b.partial, a.dlower, shares, a.D, st);
 }
 
 template <typename T, int V, bool GATE, bool PACKED>
