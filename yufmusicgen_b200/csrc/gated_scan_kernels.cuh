@@ -971,7 +971,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     const auto up = [&](auto fast) {  // fast: every token is live, and none first or last
       constexpr bool F_ = decltype(fast)::value;
       T* dgq = GATE ? static_cast<T*>(p.dg) + row0 : nullptr;
-      const auto token = [&](int j, Fv<V> xv, Fv<V> s, Fv<V> m, Fv<V> dyv, Fv<V> sgm, T* dg_at) {
+      const auto token = [&](int j, Fv<V> xv, Fv<V> s, Fv<V> m, Fv<V> dyv, Fv<V> sgm, Fv<V> mgm, T* dg_at) {
         const Fv<V> a = fma(k.om, s, k.lo);
         if constexpr (TMA) {
           put_word(sx, j, lane, m.v[0]);
@@ -989,7 +989,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         q[j] = dyv;
         if constexpr (GATE) {
           q[j] = mul(q[j], sgm);
-          const Fv<V> dg = mul(mul(q[j], h), fma(sgm, splat<V>(-1.f), splat<V>(1.f)));
+          const Fv<V> dg = mul(mul(q[j], h), mgm);
           if constexpr (OUT_SLOT) put_row<T, V>(sg, j, lane, dg);
           else if (k.act) store_raw<T, V>(dg_at, dg);
         }
@@ -1009,28 +1009,29 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
 #pragma unroll
         for (int j0 = 0; j0 < L; j0 += N) {
           Raw<T, V> xv[N], fv[N], dv[N];
-          Fv<V> s[N], m[N], sgm[N];
+          Fv<V> s[N], m[N], sgm[N], mgm[N];
           take(xv, X, j0);
           take(fv, F, j0);
           take(dv, Dy, j0);
           if constexpr (GATE) {
             Raw<T, V> gv[N];
             take(gv, Gt, j0);
-            group_gates<!RANGES>(gv, sgm);
+            group_pairs<!RANGES>(gv, sgm, mgm);
           }
           group_pairs<!RANGES>(fv, s, m);
 #pragma unroll
-          for (int u = 0; u < N; ++u, dgq += p.D) token(j0 + u, xv[u].get(), s[u], m[u], dv[u].get(), sgm[u], dgq);
+          for (int u = 0; u < N; ++u, dgq += p.D)
+            token(j0 + u, xv[u].get(), s[u], m[u], dv[u].get(), sgm[u], mgm[u], dgq);
         }
       } else {  // a row's end; pairs without slots, whose raw rows leave no registers for a group
 #pragma unroll
         for (int j = 0; j < L; ++j, dgq += p.D) {
           e[j] = q[j] = splat<V>(0.f);
           if (run.live >> j & 1) {
-            Fv<V> s, m, sgm;
+            Fv<V> s, m, sgm, mgm;
             sigmoid_pair(sigmoid_arg(F(j)).get(), s, m);
-            if constexpr (GATE) sgm = sigmoid_of(Gt(j).get());
-            token(j, X(j).get(), s, m, Dy(j).get(), sgm, dgq);
+            if constexpr (GATE) sigmoid_pair(sigmoid_arg(Gt(j)).get(), sgm, mgm);
+            token(j, X(j).get(), s, m, Dy(j).get(), sgm, mgm, dgq);
           } else if (GATE && (lanes >> j & 1)) {
             store_raw<T, V>(dgq, splat<V>(0.f));
           }
