@@ -68,3 +68,11 @@ FORMS = [(1, 60, 64), (2, 77, 33), (2, 2060, 72), (80, 130, 16), (80, 100, 17)]
 def test_output_gate_at_both_ends(B, T, D, dtype):
     """The gradient of a saturated gate keeps its relative accuracy on both sides."""
     check(make(B, T, D, dtype, seed=T, ends="gate"), ("y", "gate"))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("B,T,D", FORMS)
+def test_forget_gate_at_both_ends(B, T, D, dtype):
+    """Every gradient where the state is all but kept or all but replaced: a retention near 0
+    keeps its relative accuracy as much as an input share near 0."""
+    check(make(B, T, D, dtype, seed=T, ends="forget"))

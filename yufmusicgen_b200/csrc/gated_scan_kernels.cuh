@@ -427,13 +427,18 @@ YUF_DEVICE Fv<V> rcp_turns(Fv<V> e, int u) {
 }
 // Rates of a group of tokens, and gates of a group.
 template <bool TURNS, typename T, int V, int N>
-YUF_DEVICE void group_pairs(const Raw<T, V> (&f)[N], Fv<V> (&s)[N], Fv<V> (&m)[N]) {
+YUF_DEVICE void group_exps(const Raw<T, V> (&f)[N], Fv<V> (&s)[N], Fv<V> (&ex)[N]) {  // sigmoid(-f) = ex s
 #pragma unroll
   for (int u = 0; u < N; ++u) {
-    m[u] = sigmoid_exp(sigmoid_arg(f[u]).get());
-    s[u] = rcp_turns<TURNS>(m[u], u);
-    m[u] = mul(m[u], s[u]);
+    ex[u] = sigmoid_exp(sigmoid_arg(f[u]).get());
+    s[u] = rcp_turns<TURNS>(ex[u], u);
   }
+}
+template <bool TURNS, typename T, int V, int N>
+YUF_DEVICE void group_pairs(const Raw<T, V> (&f)[N], Fv<V> (&s)[N], Fv<V> (&m)[N]) {
+  group_exps<TURNS>(f, s, m);
+#pragma unroll
+  for (int u = 0; u < N; ++u) m[u] = mul(m[u], s[u]);
 }
 template <bool TURNS, typename T, int V, int N>
 YUF_DEVICE void group_rates(const Columns<T, V>& k, const Raw<T, V> (&f)[N], Fv<V> (&a)[N], Fv<V> (&in)[N]) {
@@ -837,10 +842,12 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
 // (one per L tokens: 1/16 of a tensor's elements).  The same pass stores dg and forms
 // the run's map G -> A G + H from its start on, H = sum_j P_j p_j with
 // P_j = a_0 ... a_j, A = P_{L-1}.  Then the tokens run from their end.
-// Slots: two stages of x and f (m = sigmoid(-f), 4 bytes a channel, is put over both
-// by the first pass, dx and df by the second; s is 1 - m there, off by 2^-25); one of
-// dy, loaded again once h has been formed; one of g, which dg is put over, loaded again
-// once dg has left.
+// Slots: two stages of x and f (e^-f, 4 bytes a channel, is put over both by the first
+// pass, dx and df by the second); one of dy, loaded again once h has been formed; one of
+// g, which dg is put over, loaded again once dg has left.  e^-f gives both sigmoid(f) and
+// sigmoid(-f) their relative accuracy again for one reciprocal, here by the special
+// function unit alone (by turns with Newton's iteration 8x2048x640 bf16 took 77.9 us
+// forward and backward, now 76.2; the smaller of the two sigmoids kept with a sign 77.7).
 // 16x8192x1024 bf16 with a gate: 347 us, 5.5 TB/s of its 1.9 GB; bound by the latency of
 // its instructions at 16 warps per SM (h and p of the run fill the registers).
 constexpr int bwd_slots(bool gate) { return gate ? 6 : 5; }
@@ -971,11 +978,11 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     const auto up = [&](auto fast) {  // fast: every token is live, and none first or last
       constexpr bool F_ = decltype(fast)::value;
       T* dgq = GATE ? static_cast<T*>(p.dg) + row0 : nullptr;
-      const auto token = [&](int j, Fv<V> xv, Fv<V> s, Fv<V> m, Fv<V> dyv, Fv<V> sgm, Fv<V> mgm, T* dg_at) {
+      const auto token = [&](int j, Fv<V> xv, Fv<V> s, Fv<V> ex, Fv<V> dyv, Fv<V> sgm, Fv<V> mgm, T* dg_at) {
         const Fv<V> a = fma(k.om, s, k.lo);
         if constexpr (TMA) {
-          put_word(sx, j, lane, m.v[0]);
-          if constexpr (V == 2) put_word(sf, j, lane, m.v[V - 1]);
+          put_word(sx, j, lane, ex.v[0]);
+          if constexpr (V == 2) put_word(sf, j, lane, ex.v[V - 1]);
         }
         if (!F_ && !(run.live >> j & 1)) {
           e[j] = q[j] = splat<V>(0.f);
@@ -985,7 +992,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         }
         if (PACKED && !F_ && (run.first >> j & 1)) h = row_of<V>(p.h0, run.owner_of(j), p.D, k.c, k.act);
         e[j] = fma(xv, splat<V>(-1.f), h);
-        h = fma(a, h, mul(mul(k.om, m), xv));
+        h = fma(a, h, mul(mul(k.om, mul(ex, s)), xv));
         q[j] = dyv;
         if constexpr (GATE) {
           q[j] = mul(q[j], sgm);
@@ -1009,7 +1016,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
 #pragma unroll
         for (int j0 = 0; j0 < L; j0 += N) {
           Raw<T, V> xv[N], fv[N], dv[N];
-          Fv<V> s[N], m[N], sgm[N], mgm[N];
+          Fv<V> s[N], ex[N], sgm[N], mgm[N];
           take(xv, X, j0);
           take(fv, F, j0);
           take(dv, Dy, j0);
@@ -1018,20 +1025,20 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
             take(gv, Gt, j0);
             group_pairs<!RANGES>(gv, sgm, mgm);
           }
-          group_pairs<!RANGES>(fv, s, m);
+          group_exps<!RANGES>(fv, s, ex);
 #pragma unroll
           for (int u = 0; u < N; ++u, dgq += p.D)
-            token(j0 + u, xv[u].get(), s[u], m[u], dv[u].get(), sgm[u], mgm[u], dgq);
+            token(j0 + u, xv[u].get(), s[u], ex[u], dv[u].get(), sgm[u], mgm[u], dgq);
         }
       } else {  // a row's end; pairs without slots, whose raw rows leave no registers for a group
 #pragma unroll
         for (int j = 0; j < L; ++j, dgq += p.D) {
           e[j] = q[j] = splat<V>(0.f);
           if (run.live >> j & 1) {
-            Fv<V> s, m, sgm, mgm;
-            sigmoid_pair(sigmoid_arg(F(j)).get(), s, m);
+            Fv<V> sgm, mgm;
+            const Fv<V> ex = sigmoid_exp(sigmoid_arg(F(j)).get()), s = rcp_1p(ex);
             if constexpr (GATE) sigmoid_pair(sigmoid_arg(Gt(j)).get(), sgm, mgm);
-            token(j, X(j).get(), s, m, Dy(j).get(), sgm, mgm, dgq);
+            token(j, X(j).get(), s, ex, Dy(j).get(), sgm, mgm, dgq);
           } else if (GATE && (lanes >> j & 1)) {
             store_raw<T, V>(dgq, splat<V>(0.f));
           }
@@ -1065,12 +1072,14 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
       T* dfq = static_cast<T*>(p.df) + row0 + (long long)(L - 1) * p.D;
 #pragma unroll
       for (int j0 = L - GROUP; j0 >= 0; j0 -= GROUP) {
-        [[maybe_unused]] Fv<V> mg[GROUP];
+        [[maybe_unused]] Fv<V> sv[GROUP], mv[GROUP];
         if constexpr (TMA) {
 #pragma unroll
           for (int u = 0; u < GROUP; ++u) {
-            mg[u].v[0] = get_word(sx, j0 + u, lane);
-            if constexpr (V == 2) mg[u].v[V - 1] = get_word(sf, j0 + u, lane);
+            mv[u].v[0] = get_word(sx, j0 + u, lane);
+            if constexpr (V == 2) mv[u].v[V - 1] = get_word(sf, j0 + u, lane);
+            sv[u] = rcp_1p(mv[u]);
+            mv[u] = mul(mv[u], sv[u]);
           }
         }
 #pragma unroll
@@ -1081,8 +1090,8 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
             if (PACKED && !F_ && (run.last >> j & 1)) Gw = row_of<V>(p.dh_last, run.owner_of(j), p.D, k.c, k.act);
             Fv<V> s, m;
             if constexpr (TMA) {
-              m = mg[u];
-              s = fma(m, splat<V>(-1.f), splat<V>(1.f));
+              s = sv[u];
+              m = mv[u];
             } else {
               sigmoid_pair(sigmoid_arg(fr[j]).get(), s, m);
             }
@@ -1118,7 +1127,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         bulk_commit();
       }
     } else if constexpr (TMA) {
-      fence_proxy_async();  // m was put over the slots
+      fence_proxy_async();  // e^-f was put over the slots
       __syncwarp();
       if (lane == 0) issue_xf(i + 2);
     }
