@@ -76,3 +76,24 @@ def test_forget_gate_at_both_ends(B, T, D, dtype):
     """Every gradient where the state is all but kept or all but replaced: a retention near 0
     keeps its relative accuracy as much as an input share near 0."""
     check(make(B, T, D, dtype, seed=T, ends="forget"))
+
+
+@pytest.mark.parametrize("copies", [False, True])
+def test_dlower_sums_many_equal_terms(copies):
+    """2.6 million terms of nearly the same size per channel: an fp32 sum of them drops the
+    same bits of each one again and again.  The rows of the batch are alike, so the sum is
+    B times that of one row (``copies``: rows of their own, or shared ones)."""
+    B, T, D = 80, 32768, 32
+    size = torch.arange(1, D + 1, device=DEV) / D + 0.37
+    sign = 1 - 2.0 * (torch.arange(T, device=DEV) % 2)
+    x = (sign[:, None] * size)[None]
+    v = {"x": x, "forget": torch.linspace(-2, 2, D, device=DEV).expand(1, T, D), "gate": None,
+         "lower": torch.zeros(D, device=DEV), "state": None, "dy": x, "dlast": torch.zeros(1, D, device=DEV)}
+    want, bound = gb.gated_scan_bounds(*(f64(v[k]) for k in NAMES), None, f64(v["dy"]), f64(v["dlast"]))
+    rows = {k: v[k].expand(B, T, D) for k in ("x", "forget", "dy")}
+    if copies:
+        rows = {k: t.contiguous() for k, t in rows.items()}
+    lower = v["lower"].requires_grad_(True)
+    y, _ = gated_scan(rows["x"], rows["forget"], None, lower)
+    (g,) = torch.autograd.grad(y, lower, rows["dy"])
+    assert gb.beyond(f64(g), B * want["lower"], B * bound["lower"]) <= 0

@@ -55,14 +55,14 @@ bool gated_scan_pairs(const GatedScanArgs& a) {
 
 namespace {
 
-// dlower[c] = sum over rows of partial[rows, D], in a fixed order: 32 warps a block,
+// dlower[c] = sum over rows of partial[rows, D], in 64 bits and a fixed order: 32 warps a block,
 // each every 32nd row, as many loads under way as there are rows (592 rows: 5 us with
 // 8 warps)
 __global__ void __launch_bounds__(1024)
     gated_scan_dlower_kernel(const float* __restrict__ partial, float* __restrict__ out, long long rows, int D) {
-  __shared__ float part[32][33];
+  __shared__ double part[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  float sum = 0.f;
+  double sum = 0.;
   if (c < D) {
 #pragma unroll 4
     for (long long r = w; r < rows; r += 32) sum += partial[r * D + c];
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(1024)
   sum = part[lane][w];  // warp w: channel w of the block
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0 && blockIdx.x * 32 + w < D) out[blockIdx.x * 32 + w] = sum;
+  if (lane == 0 && blockIdx.x * 32 + w < D) out[blockIdx.x * 32 + w] = (float)sum;
 }
 
 // ---------------------------------------------------------------------------

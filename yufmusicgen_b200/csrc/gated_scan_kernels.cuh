@@ -150,6 +150,7 @@ YUF_DEVICE void linger(const Place& q) {
 // behind a barrier that every reader has passed).
 constexpr int join_bytes(int V, int nw) { return 2 * 32 * V * (8 * nw + 4); }
 constexpr int maps_bytes(int V, int nw) { return 32 * V * 8 * nw; }  // of ranges: one copy of the maps
+constexpr int sums_bytes(int V, int nw) { return 32 * V * 8 * nw; }  // of dlower, a double per lane and channel
 template <int V>
 struct Joint {
   float2* warp_;
@@ -853,18 +854,19 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
 constexpr int bwd_slots(bool gate) { return gate ? 6 : 5; }
 
 // The block's share of dlower, the sum over its warps, to row `row` of `partial`.
+// dlower sums over all tokens and rows: in fp32 within a run only, its 16 terms; runs,
+// warps and blocks are added in 64 bits, where rounding does not grow with their number.
 template <int V>
-YUF_DEVICE void write_partial(const Joint<V>& m, const GatedScanArgs& p, const Place& q, Fv<V> dlo, long long row,
-                              int c, bool act) {
-  __syncthreads();
-  float* const part = &m.warp(0, 0)->x;
-  store_f32<V>(part + (q.w * 32 + q.lane) * V, dlo);
+YUF_DEVICE void write_partial(const double* sums, const GatedScanArgs& p, const Place& q, long long row, int c,
+                              bool act) {
   __syncthreads();
   if (q.w == 0 && act) {
-    Fv<V> sum = splat<V>(0.f);
-    for (int k = 0; k < q.nw; ++k) sum = add(sum, load_f32<V>(part + (k * 32 + q.lane) * V));
 #pragma unroll
-    for (int i = 0; i < V; ++i) p.partial[row * p.D + c + i] = sum.v[i];
+    for (int i = 0; i < V; ++i) {
+      double sum = 0.;
+      for (int k = 0; k < q.nw; ++k) sum += sums[(k * V + i) * 32 + q.lane];
+      p.partial[row * p.D + c + i] = (float)sum;
+    }
   }
 }
 
@@ -877,7 +879,18 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
   extern __shared__ __align__(128) char smem[];
   Place at = range_place<true>(sp);
   const int lane = at.lane, w = threadIdx.x >> 5, nw = at.nw;
-  const Joint<V> joint(smem + (TMA ? nw * (bwd_slots(GATE) * SLOT + 32) : 0), nw);
+  constexpr int PER_WARP = TMA ? bwd_slots(GATE) * SLOT + 32 : 0;
+  const Joint<V> joint(smem + nw * PER_WARP, nw);
+  // The warps' sums of dlower: of packed rows, whose kernels have no register left, in
+  // shared memory of their own (forward and backward of packed 8192x4096 bf16: 298 us
+  // against 314), otherwise in registers until the end (1x16384x1024: 105 against 111).
+  double* const sums = reinterpret_cast<double*>(
+      smem + nw * PER_WARP + (!PACKED ? 0 : RANGES ? maps_bytes(V, nw) : join_bytes(V, nw)));
+  double* const my_sum = sums + w * V * 32 + lane;
+  double dlo[V] = {};
+  if (PACKED && p.partial)
+#pragma unroll
+    for (int u = 0; u < V; ++u) my_sum[u * 32] = 0.;
   const Columns<T, V> k(p, at.col, sp.n_cblk, lane);
   const T* const xp = row_ptr<T>(p.x, p.xb, k.b, k.c);
   const T* const fp = row_ptr<T>(p.f, p.fb, k.b, k.c);
@@ -921,7 +934,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
   }
   Run run{};
   look<PACKED, true>(run, p, t_of(0), lane);  // while the first loads are under way
-  Fv<V> G = splat<V>(0.f), dlo = splat<V>(0.f);
+  Fv<V> G = splat<V>(0.f);
   if constexpr (PACKED) {
     if (p.dh0 && k.act) empty_sequences<V>(p, p.dh_last, p.dh0, k.c, at.chunk * nw + w, sp.chunks * nw);
   } else {
@@ -1066,6 +1079,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
       bulk_wait_read<0>();
       issue_one(i + 1, sg, &tm.g, &full[3]);
     }
+    Fv<V> dl = splat<V>(0.f);  // this run's share of dlower
     const auto down = [&](auto fast) {
       constexpr bool F_ = decltype(fast)::value;
       T* dxq = static_cast<T*>(p.dx) + row0 + (long long)(L - 1) * p.D;
@@ -1098,7 +1112,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
             const Fv<V> dh = add(q[j], Gw), dhm = mul(dh, m);
             dx = mul(dhm, k.om);
             df = mul(mul(dx, e[j]), s);
-            dlo = fma(dhm, e[j], dlo);
+            dl = fma(dhm, e[j], dl);
             Gw = mul(fma(k.om, s, k.lo), dh);
             if (PACKED && !F_ && (run.first >> j & 1)) {
               const int o = run.owner_of(j);
@@ -1117,6 +1131,14 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     };
     if (plain) down(std::true_type{});
     else down(std::false_type{});
+    if constexpr (PACKED) {
+      if (p.partial)
+#pragma unroll
+        for (int u = 0; u < V; ++u) my_sum[u * 32] += dl.v[u];
+    } else {
+#pragma unroll
+      for (int u = 0; u < V; ++u) dlo[u] += dl.v[u];
+    }
     if constexpr (RANGES) G = Gw;
     if constexpr (OUT_SLOT) {
       fence_proxy_async();
@@ -1134,7 +1156,12 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
   }
   // G_0: of the whole form in its last warp, of ranges where token 0 is
   if (!PACKED && p.dh0 && k.act && (RANGES ? r0 == 0 : w == 0)) store_f32<V>(p.dh0 + (long long)k.b * p.D + k.c, G);
-  if (p.partial) write_partial<V>(joint, p, at, dlo, (long long)k.b * sp.chunks + blockIdx.x % sp.chunks, k.c, k.act);
+  if (!PACKED && p.partial) {
+    __syncthreads();  // the maps in this place have been read
+#pragma unroll
+    for (int u = 0; u < V; ++u) my_sum[u * 32] = dlo[u];
+  }
+  if (p.partial) write_partial<V>(sums, p, at, (long long)k.b * sp.chunks + blockIdx.x % sp.chunks, k.c, k.act);
   if (OUT_SLOT && lane == 0) bulk_wait_read<0>();
   if constexpr (TMA) linger(at);
 }
@@ -1243,7 +1270,8 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
 // ---- host -------------------------------------------------------------------
 
 constexpr int SMEM_MAX = 227 * 1024;
-static_assert(NW_MAX * (bwd_slots(true) * SLOT + 32) + join_bytes(2, NW_MAX) <= SMEM_MAX, "shared memory of a block");
+static_assert(NW_MAX * (bwd_slots(true) * SLOT + 32) + join_bytes(2, NW_MAX) + sums_bytes(2, NW_MAX) <= SMEM_MAX,
+              "shared memory of a block");
 
 // A kernel's dynamic shared memory, allowed once per device.
 bool allow_smem(const void* kernel, std::atomic<uint64_t>& done) {
@@ -1337,7 +1365,7 @@ template <typename T, int V, bool GATE, bool PACKED, bool TMA>
 yuf_status_t backward_with(const GatedScanArgs& a, const ScanMaps& m, cudaStream_t st) {
   const Plan p = gated_scan_plan(a.B, a.T, a.D, V);
   const int j = p.ranges ? maps_bytes(V, p.nw) : join_bytes(V, p.nw);
-  const int s = (TMA ? p.nw * (bwd_slots(GATE) * SLOT + 32) : 0) + j;
+  const int s = (TMA ? p.nw * (bwd_slots(GATE) * SLOT + 32) : 0) + j + (PACKED ? sums_bytes(V, p.nw) : 0);
   GatedScanArgs b = a;
   const long long shares = (long long)a.B * p.sp.chunks;  // of dlower
   if (a.dlower) b.partial = shares == 1 ? a.dlower : a.work + p.map_floats(V);
