@@ -67,6 +67,17 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// Derivatives in forward mode are not there: a tangent must not get lost in silence.
+void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    NEED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), NotImplementedError, name,
+         " has no forward-mode derivatives (an input has a tangent)");
+}
+void no_tangents(const char* name, const variable_list& grads) {  // of a backward
+  for (const Tensor& t : grads)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
+                                " has no forward-mode derivatives (a gradient has a tangent)");
+}
 // A failing library call (the message of its thread).
 void check(const char* name, yuf_status_t st) {
   TORCH_CHECK(st == YUF_OK, name, " failed with ", yuf_status_string(st), ": ", yuf_last_error());
@@ -179,6 +190,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool recorded = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
+    no_tangents("gated_scan", grads);
     const auto saved = ctx->get_saved_variables();
     const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], dtype_of(saved[0]),
                     ctx->saved_data["rows"].toInt()};
@@ -257,6 +269,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool recorded = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
+    no_tangents("dropout", grads);
     const auto draw = ctx->saved_data["draw"].toIntVector();
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
@@ -312,6 +325,7 @@ PyObject* py_gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* names[] = {"x", "forget", "gate", "lower", "state", "cu_seqlens"};
     Tensor t[6];
     for (int i = 0; i < 6; ++i) t[i] = tensor_of(a[i], names[i]);
+    no_tangents("gated_scan", {&t[0], &t[1], &t[2], &t[3], &t[4]});
     check_tokens(t[0], t[1], t[2], t[3], 3);
     const int64_t rows = check_states(t[0], t[4], t[5]);
     for (int i = 0; i < 3; ++i) t[i] = unit_rows(t[i]);
@@ -341,6 +355,7 @@ PyObject* py_gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Tensor x = tensor_of(a[0], "x"), f = tensor_of(a[1], "forget"), state = tensor_of(a[2], "state"),
            g = tensor_of(a[3], "gate"), lower = tensor_of(a[4], "lower");
+    no_tangents("gated_scan_step", {&x, &f, &state, &g, &lower});
     check_tokens(x, f, g, lower, 2);
     NEED(state.defined() && state.scalar_type() == at::kFloat, TypeError, "gated scan: state must be float32");
     NEED(state.sizes() == x.sizes() && state.device() == x.device(), ValueError,
@@ -370,6 +385,7 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 5, "dropout")) return nullptr;
   return guarded([&]() -> PyObject* {
     const Tensor x = tensor_of(a[0], "dropout: x"), r = tensor_of(a[4], "dropout: residual");
+    no_tangents("dropout", {&x, &r});
     NEED(x.defined() && x.is_cuda(), ValueError, "dropout: x must be on CUDA");
     NEED(dtype_of(x) >= 0, TypeError, "dropout: x must be float32, bfloat16 or float16, got ", x.scalar_type());
     const double p = PyFloat_AsDouble(a[1]);

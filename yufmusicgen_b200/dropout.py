@@ -26,5 +26,6 @@ def dropout(x, p, seed, step=0, residual=None):
     element, read when the kernel runs (advance it between replays of a captured
     training step).  It must not change between the forward and the backward.
 
-    Raises ValueError or TypeError for what the kernels do not take."""
+    Raises ValueError or TypeError for what the kernels do not take, NotImplementedError for
+    an input with a forward-mode tangent."""
     return ops.dropout(x, p, seed, step, residual)

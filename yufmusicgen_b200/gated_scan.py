@@ -38,12 +38,13 @@ def gated_scan(x, forget, gate=None, lower=None, state=None, cu_seqlens=None):
     The contents of ``cu_seqlens`` are not checked (that would wait for the GPU).
 
     Raises ValueError or TypeError for what the kernels do not take.  The gradients
-    cannot be differentiated again (RuntimeError where that is tried)."""
+    cannot be differentiated again (RuntimeError where that is tried), and there are no
+    forward-mode derivatives (NotImplementedError for an input with a tangent)."""
     return ops.gated_scan(x, forget, gate, lower, state, cu_seqlens)
 
 
 def gated_scan_step(x, forget, state, gate=None, lower=None):
     """One token of ``B`` sequences: ``x``, ``forget``, ``gate`` ``[B, D]``; ``state
     [B, D]`` (float32, e.g. a row range of a pool of states) is updated in place.
-    Returns ``y [B, D]``.  Not differentiable."""
+    Returns ``y [B, D]``.  Not differentiable (NotImplementedError where that is asked for)."""
     return ops.gated_scan_step(x, forget, state, gate, lower)
