@@ -234,7 +234,8 @@ yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const vo
                                      void* workspace, int dtype, int B, int T, int D, void* stream);
 /* One token of B sequences: x, forget, gate (or NULL) [B, D] with row strides
  * strides [3] (NULL = contiguous), y [B, D] contiguous; state [B, D] fp32 with row
- * stride state_stride (>= D) is updated in place, e.g. a slot range of a pool. */
+ * stride state_stride (>= D) is updated in place, e.g. a slot range of a pool.
+ * B D <= 2^38. */
 yuf_status_t yuf_gated_scan_step(const void* x, const void* forget, const void* gate,
                                  const int64_t* strides, const float* lower, float* state,
                                  int64_t state_stride, void* y, int dtype, int B, int D,
@@ -251,7 +252,7 @@ yuf_status_t yuf_gated_scan_step(const void* x, const void* forget, const void* 
  * Types (x, out): equal ones; bf16 or fp16 x with fp32 out (an fp32 residual
  * stream); fp32 x with bf16 or fp16 out and no residual (that call's gradient).
  * step_device (device, 8 bytes), when not NULL, is read instead of `step`, so a
- * captured graph draws new masks as the caller advances it. */
+ * captured graph draws new masks as the caller advances it.  rows cols <= 2^40. */
 yuf_status_t yuf_dropout(const void* x, int64_t x_stride, int x_dtype, const void* residual,
                          int64_t residual_stride, void* out, int out_dtype, int64_t rows,
                          int64_t cols, double p, uint64_t seed, uint64_t step,

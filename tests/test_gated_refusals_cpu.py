@@ -27,3 +27,19 @@ def test_forward_mode_tangents_are_refused(requires_grad):
                     call(**{**args, k: dual})
                 with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
                     call(**{**args, k: dual})
+
+
+def test_sizes_beyond_the_limits_are_value_errors():
+    """Refused before an output is allocated (the tensors here are one element, shared)."""
+    one = torch.zeros(1, 1, 1)
+    for shape in ((1, 2**30 + 1, 1), (2**26 + 1, 1, 1), (1, 1, 2**31), (2**20, 1, 32 * 64 + 1)):
+        with pytest.raises(ValueError, match="too large"):
+            gated_scan(one.expand(shape), one.expand(shape))
+    big = one[0].expand(2**20, 2**18 + 1)
+    with pytest.raises(ValueError, match="too large"):
+        gated_scan_step(big, big, big)
+    with pytest.raises(ValueError, match="too large"):
+        dropout(one.expand(2**20, 2**10, 2**10 + 1), 0.5, 1)
+    for shape in ((1, 2**30, 1), (2**26, 1, 1), (2**20, 1, 32 * 64)):  # at the limits
+        with pytest.raises(ValueError, match="CUDA"):
+            gated_scan(one.expand(shape), one.expand(shape))

@@ -116,18 +116,24 @@ void check_tokens(const Tensor& x, const Tensor& f, const Tensor& g, const Tenso
   NEED(x.defined() && f.defined(), TypeError, "gated scan: x and forget must be tensors");
   NEED(x.dim() == ndim, ValueError, "gated scan: x must have shape ", ndim == 3 ? "[B, T, D]" : "[B, D]", ", got ",
        x.sizes());
-  NEED(x.is_cuda(), ValueError, "gated scan inputs must be on CUDA");
   NEED(dtype_of(x) >= 0, TypeError, "gated scan: x must be float32, bfloat16 or float16, got ", x.scalar_type());
   for (const Tensor* t : {&f, &g})
     NEED(!t->defined() || (t->sizes() == x.sizes() && t->scalar_type() == x.scalar_type() && t->device() == x.device()),
          ValueError, "gated scan: ", t == &f ? "forget" : "gate", " must have x's shape, type and device");
   NEED(x.size(-1) >= 1, ValueError, "gated scan: D must be at least 1");
-  for (int64_t n : x.sizes()) NEED(n <= INT32_MAX, ValueError, "gated scan: x is too large: ", x.sizes());
+  // the library's own limits, before anything is allocated
+  bool fits = true;
+  for (int64_t n : x.sizes()) fits = fits && n <= INT32_MAX;
+  const int64_t B = x.size(0), D = x.size(-1);
+  if (ndim == 3) fits = fits && x.size(1) <= (int64_t{1} << 30) && B * ((D + 31) / 32) <= (int64_t{1} << 26);
+  else fits = fits && B * D <= (int64_t{1} << 38);
+  NEED(fits, ValueError, "gated scan: x is too large: ", x.sizes());
   if (lower.defined()) {
     NEED(lower.scalar_type() == at::kFloat, TypeError, "gated scan: lower must be float32");
     NEED(lower.dim() == 1 && lower.size(0) == x.size(-1) && lower.device() == x.device(), ValueError,
          "gated scan: lower must be a [D] tensor on x's device");
   }
+  NEED(x.is_cuda(), ValueError, "gated scan inputs must be on CUDA");
 }
 
 int64_t check_states(const Tensor& x, const Tensor& state, const Tensor& cu) {
@@ -386,7 +392,7 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const Tensor x = tensor_of(a[0], "dropout: x"), r = tensor_of(a[4], "dropout: residual");
     no_tangents("dropout", {&x, &r});
-    NEED(x.defined() && x.is_cuda(), ValueError, "dropout: x must be on CUDA");
+    NEED(x.defined(), TypeError, "dropout: x must be a tensor, got None");
     NEED(dtype_of(x) >= 0, TypeError, "dropout: x must be float32, bfloat16 or float16, got ", x.scalar_type());
     const double p = PyFloat_AsDouble(a[1]);
     if (p == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
@@ -397,6 +403,8 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
       NEED(r.scalar_type() == x.scalar_type() || r.scalar_type() == at::kFloat, TypeError,
            "dropout: residual must have x's type or be float32");
     }
+    NEED(x.numel() <= (int64_t{1} << 40), ValueError, "dropout: x is too large: ", x.sizes());
+    NEED(x.is_cuda(), ValueError, "dropout: x must be on CUDA");
     Draw d{p, word_of(a[2]), 0};
     Tensor step_t;
     if (THPVariable_Check(a[3])) {
