@@ -31,3 +31,40 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(NotImplementedError, match="tangent"):
                 torch.autograd.grad(loss, leaf)
     assert torch.isfinite(gated_scan(x, f)[0]).all()
+
+
+def lazily_negated(*shape):
+    """A float32 tensor that torch negates only when it is read (the imaginary part of a
+    conjugate), with a last axis of one element: no copy for the sake of its strides."""
+    t = torch.randn(*shape, 1, dtype=torch.complex64, device=DEV).conj().imag
+    assert t.is_neg() and t.dtype == torch.float32
+    return t
+
+
+def test_lazily_negated_tensors():
+    x, f, g, h0, dy, dl = *(lazily_negated(2, 40) for _ in range(3)), lazily_negated(2), lazily_negated(2, 40), lazily_negated(2)
+    low = torch.full((1,), -0.5j, device=DEV).conj().imag
+    plain = [t.clone() for t in (x, f, g, low, h0)]
+    assert float(low) == 0.5 and low.is_neg() and not any(t.is_neg() for t in plain)
+    for a, b in zip(gated_scan(x, f, g, low, h0), gated_scan(*plain)):
+        assert torch.equal(a, b)
+    leaves = [t.requires_grad_(True) for t in plain]
+    out = gated_scan(*leaves)
+    for a, b in zip(torch.autograd.grad(out, leaves, (dy, dl), retain_graph=True),
+                    torch.autograd.grad(out, leaves, (dy.clone(), dl.clone()))):
+        assert torch.equal(a, b)
+    s1, s2 = (torch.zeros(2, 1, device=DEV) for _ in range(2))
+    y = gated_scan_step(x[:, 0], f[:, 0], s1, g[:, 0], low)
+    assert torch.equal(y, gated_scan_step(*(t[:, 0].clone() for t in (x, f)), s2, g[:, 0].clone(), low.clone()))
+    assert torch.equal(s1, s2)
+    with pytest.raises(ValueError, match="negated"):
+        gated_scan_step(x[:, 0], f[:, 0], h0)
+
+
+def test_lazily_negated_tensors_in_dropout():
+    x, r, dy = (lazily_negated(50) for _ in range(3))
+    assert torch.equal(dropout(x, 0.25, 3, 4, r), dropout(x.clone(), 0.25, 3, 4, r.clone()))
+    leaf = x.detach().clone().requires_grad_(True)
+    (a,) = torch.autograd.grad(dropout(leaf, 0.25, 3), leaf, dy)
+    (b,) = torch.autograd.grad(dropout(leaf, 0.25, 3), leaf, dy.clone())
+    assert torch.equal(a, b)

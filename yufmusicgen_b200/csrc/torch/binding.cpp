@@ -52,11 +52,14 @@ template <typename T>
 T* ptr(const Tensor& t) {
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
+// the values as they lie in memory (a copy where torch negates them only when it reads them)
+Tensor as_stored(const Tensor& t) { return t.defined() ? t.resolve_neg() : t; }
 // a unit stride along the last axis (a copy where it has none)
-Tensor unit_rows(const Tensor& t) {
+Tensor unit_rows(const Tensor& u) {
+  const Tensor t = as_stored(u);
   return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
-Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor dense(const Tensor& t) { return t.defined() ? as_stored(t).contiguous() : t; }
 // Arguments of an autograd node that may be absent.
 using Maybe = std::optional<Tensor>;
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
@@ -246,6 +249,8 @@ struct Draw {
 // step_t, where defined, holds the step on the device
 Tensor drop(Tensor x, Tensor r, const Draw& d, const Tensor& step_t, at::ScalarType out_type) {
   On on(x);
+  x = as_stored(x);
+  r = as_stored(r);
   const Tensor out = at::empty(x.sizes(), x.options().dtype(out_type).memory_format(at::MemoryFormat::Contiguous));
   int64_t rows = 1, cols = x.numel(), xs = cols, rs = cols;
   if (x.dim() > 0 && x.numel() > 0 && !(x.is_contiguous() && (!r.defined() || r.is_contiguous()))) {
@@ -369,6 +374,7 @@ PyObject* py_gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t B = x.size(0), D = x.size(1);
     NEED((D == 1 || state.stride(1) == 1) && (B <= 1 || state.stride(0) >= D), ValueError,
          "gated scan: state rows must be contiguous and must not overlap");
+    NEED(!state.is_neg(), ValueError, "gated scan: state must not be a lazily negated view");
     NEED(!wants_grad({&x, &f, &g, &lower, &state}), NotImplementedError,
          "gated_scan_step has no gradients: use gated_scan, or torch.no_grad()");
     x = unit_rows(x);
