@@ -43,3 +43,36 @@ def test_sizes_beyond_the_limits_are_value_errors():
     for shape in ((1, 2**30, 1), (2**26, 1, 1), (2**20, 1, 32 * 64)):  # at the limits
         with pytest.raises(ValueError, match="CUDA"):
             gated_scan(one.expand(shape), one.expand(shape))
+
+
+def test_a_state_that_overlaps_an_input_is_refused():
+    """The step reads its inputs while it writes the state: shared memory is allowed only
+    element by element."""
+    B, D = 4, 6
+    pool, other = torch.zeros(B + 3, D), torch.zeros(B, D)
+    wide = torch.zeros(B + 2, 3 * D + 1)
+
+    def refused(word, x, f, state, gate=None, lower=None):
+        with pytest.raises(ValueError, match=word):
+            gated_scan_step(x, f, state, gate, lower)
+
+    state = pool[1:B + 1]
+    for bad in (pool[:B], pool[2:B + 2], pool[3:B + 3], pool[2:3].expand(B, D), pool.view(-1)[D + 1:].as_strided((B, D), (D, 1)),
+                pool.view(-1).as_strided((B, D), (D - 1, 1))):
+        refused("share memory", bad, other, state)
+        refused("share memory", other, bad, state)
+        refused("share memory", other, other, state, bad)
+    refused("share memory", other, other, state, None, pool[2])
+    refused("share memory", wide[:B, :D], other, wide[1:B + 1, :D])
+    refused("share memory", wide[:B, 1:D + 1], other, wide[:B, :D])
+    refused("share memory", other[:1], other[:1], pool[:1], None, pool.view(-1)[1:D + 1])
+    refused("share memory", wide.view(-1).as_strided((3, 2), (7, 1), 4), torch.zeros(3, 2), wide.view(-1).as_strided((3, 2), (14, 1), 10))
+    half = torch.zeros(B, D, dtype=torch.bfloat16)
+    refused("share memory", other.view(torch.bfloat16)[:, :D], half, other)
+    # nothing shared, or each element with itself: the next check answers
+    for x, f, st, lower in ((state, other, state, None), (pool[:1], other[:1], pool[1:2], pool[2]), (state, state, state, pool[0]),
+                            (wide[:B, :D], wide[:B, D:2 * D], wide[:B, 2 * D:3 * D], wide[B, :D]),
+                            (pool[5:6].expand(2, D), other[:2], pool[3:5], pool[2]), (pool[:2], other[:2], pool[2:4], pool[4]),
+                            (wide.view(-1).as_strided((3, 2), (7, 1), 4), torch.zeros(3, 2), wide.view(-1).as_strided((3, 2), (14, 1), 9), None),
+                            (pool[2:3], other[:1], pool[2:3], pool[2]), (pool[:0], other[:0], pool[:0], None)):
+        refused("CUDA", x, f, st, None, lower)

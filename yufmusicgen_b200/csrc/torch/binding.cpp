@@ -136,8 +136,8 @@ void check_tokens(const Tensor& x, const Tensor& f, const Tensor& g, const Tenso
     NEED(lower.dim() == 1 && lower.size(0) == x.size(-1) && lower.device() == x.device(), ValueError,
          "gated scan: lower must be a [D] tensor on x's device");
   }
-  NEED(x.is_cuda(), ValueError, "gated scan inputs must be on CUDA");
 }
+void check_cuda(const Tensor& x) { NEED(x.is_cuda(), ValueError, "gated scan inputs must be on CUDA"); }
 
 int64_t check_states(const Tensor& x, const Tensor& state, const Tensor& cu) {
   int64_t rows = x.size(0);
@@ -155,6 +155,26 @@ int64_t check_states(const Tensor& x, const Tensor& state, const Tensor& cu) {
          ValueError, "gated scan: state must be a [", rows, ", ", x.size(2), "] tensor on x's device");
   }
   return rows;
+}
+
+// Whether an input (rows along its first axis, or one row) shares memory with the state
+// that a step updates in place, other than element by element.
+bool clashes(const Tensor& state, const Tensor& t) {
+  if (!t.defined() || state.numel() == 0) return false;
+  const int64_t ws = state.size(-1) * state.itemsize(), wt = t.size(-1) * t.itemsize(), nt_ = t.dim() == 2 ? t.size(0) : 1,
+                ss = state.stride(0) * state.itemsize(), ts = nt_ > 1 ? t.stride(0) * t.itemsize() : 0,
+                ns = state.size(0), nt = ts == 0 ? 1 : nt_;  // a shared row is one row
+  const int64_t d = (int64_t)((intptr_t)t.data_ptr() - (intptr_t)state.data_ptr());
+  if (t.size(-1) > 1 && t.stride(-1) != 1)  // copied first
+    return false;
+  if (d >= (ns - 1) * ss + ws || d + (nt - 1) * ts + wt <= 0) return false;
+  if (d == 0 && ws == wt && ns == nt && (ns == 1 || ss == ts)) return false;
+  for (int64_t i = 0; i < ns; ++i) {  // rows that lie among one another: each row of the state
+    const int64_t at = i * ss - d, end = at - wt;  // its first byte behind t's; t's rows that end before it
+    const int64_t j = ts == 0 || end < 0 ? 0 : end / ts + 1;
+    if (j < nt && j * ts < at + ws && j * ts + wt > at) return true;
+  }
+  return false;
 }
 
 Tensor workspace(const Inputs& in, bool backward) {
@@ -339,6 +359,7 @@ PyObject* py_gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     no_tangents("gated_scan", {&t[0], &t[1], &t[2], &t[3], &t[4]});
     check_tokens(t[0], t[1], t[2], t[3], 3);
     const int64_t rows = check_states(t[0], t[4], t[5]);
+    check_cuda(t[0]);
     for (int i = 0; i < 3; ++i) t[i] = unit_rows(t[i]);
     t[3] = dense(t[3]);
     t[4] = dense(t[4]);
@@ -377,6 +398,9 @@ PyObject* py_gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     NEED(!state.is_neg(), ValueError, "gated scan: state must not be a lazily negated view");
     NEED(!wants_grad({&x, &f, &g, &lower, &state}), NotImplementedError,
          "gated_scan_step has no gradients: use gated_scan, or torch.no_grad()");
+    for (const Tensor* t : {&x, &f, &g, &lower})
+      NEED(!clashes(state, *t), ValueError, "gated scan: state must not share memory with other elements of an input");
+    check_cuda(x);
     x = unit_rows(x);
     f = unit_rows(f);
     g = unit_rows(g);
