@@ -1,5 +1,6 @@
-"""Build recipe for ``libyufb200.so`` (sm_100a only) and ``_yuf_torch.so``, the
-Python module that calls it on torch tensors.
+"""Build recipe for ``libyufb200.so`` (sm_100a only) and ``_yuf_torch``, the Python
+module that calls it on torch tensors (one per Python; not built where torch is missing,
+which the library does without).
 
 Each ``csrc/*.cu`` / ``*.cpp`` file is compiled to an object under
 ``yufmusicgen_b200/_build/`` (in parallel, skipped when up to date) and linked
@@ -23,7 +24,7 @@ CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_build"
 LIB = PKG / "libyufb200.so"
 TORCH_SRC = CSRC / "torch" / "binding.cpp"
-TORCH_MODULE = PKG / "_yuf_torch.so"
+TORCH_MODULE = PKG / ("_yuf_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -61,17 +62,14 @@ def _compile(src: Path, ptxas_verbose: bool) -> tuple[Path, str]:
     return obj, p.stderr
 
 
-def _torch_dir() -> Path:
+def _torch_dir() -> Path | None:
     spec = importlib.util.find_spec("torch")  # found, not imported
-    if spec is None or spec.origin is None:
-        raise RuntimeError("torch not found; it is required to build _yuf_torch")
-    return Path(spec.origin).parent
+    return Path(spec.origin).parent if spec is not None and spec.origin is not None else None
 
 
-def _compile_torch() -> Path:
+def _compile_torch(torch_dir: Path) -> Path:
     """Compile the torch module's object (it is linked once the library is there)."""
-    obj = OUT_DIR / "torch_binding.o"
-    torch_dir = _torch_dir()
+    obj = OUT_DIR / TORCH_MODULE.with_suffix(".o").name
     newest = max(TORCH_SRC.stat().st_mtime, (INCLUDE / "yufb200.h").stat().st_mtime,
                  (torch_dir / "version.py").stat().st_mtime)
     if obj.exists() and obj.stat().st_mtime >= newest:
@@ -86,12 +84,12 @@ def _compile_torch() -> Path:
     return obj
 
 
-def _link_torch(obj: Path) -> None:
+def _link_torch(obj: Path, torch_dir: Path) -> None:
     if TORCH_MODULE.exists() and TORCH_MODULE.stat().st_mtime >= obj.stat().st_mtime:
         return
     tmp = TORCH_MODULE.with_suffix(".so.tmp")
     cmd = ["g++", "-shared", "-o", str(tmp), str(obj), "-L", str(PKG), "-lyufb200", "-Wl,-rpath,$ORIGIN",
-           "-L", str(_torch_dir() / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"]
+           "-L", str(torch_dir / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"link of {TORCH_MODULE.name} failed:\n{p.stdout}\n{p.stderr}")
@@ -101,10 +99,10 @@ def _link_torch(obj: Path) -> None:
 def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     srcs = _sources()
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        torch_obj = ex.submit(_compile_torch)
+    torch_dir = _torch_dir()
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        torch_obj = ex.submit(_compile_torch, torch_dir) if torch_dir else None
         results = list(ex.map(lambda s: _compile(s, ptxas_verbose), srcs))
-        torch_obj = torch_obj.result()
     objs = [o for o, _ in results]
     if verbose:
         for o, log in results:
@@ -118,7 +116,10 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n{p.stdout}\n{p.stderr}")
         os.replace(tmp, LIB)
-    _link_torch(torch_obj)
+    if torch_obj is None:
+        print("torch not found: _yuf_torch (gated_scan, dropout) is not built", file=sys.stderr)
+    else:
+        _link_torch(torch_obj.result(), torch_dir)  # its failure is raised here, with the library in place
     return LIB
 
 
