@@ -97,3 +97,38 @@ def test_dlower_sums_many_equal_terms(copies):
     y, _ = gated_scan(rows["x"], rows["forget"], None, lower)
     (g,) = torch.autograd.grad(y, lower, rows["dy"])
     assert gb.beyond(f64(g), B * want["lower"], B * bound["lower"]) <= 0
+
+
+SHAPES = [(1, 1, 1), (2, 129, 40), (2, 1025, 66), (1, 2048, 640), (5, 64, 31), (300, 3, 10), (2, 2060, 72),
+          (37, 300, 64), (80, 530, 16), (150, 290, 8), (80, 300, 17)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("B,T,D", SHAPES)
+def test_every_element(B, T, D, dtype):
+    """Both forms, one and several steps and ranges, many batch rows."""
+    check(make(B, T, D, dtype, seed=B + T + D))
+
+
+PACKED = [([0, 5000, 5001, 8990], 9000), ([0, 200, 200, 257, 260], 270), ([0, 1, 2, 3], 3), ([0, 127, 129, 129, 1000], 1100)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 37])
+@pytest.mark.parametrize("cu,T", PACKED)
+def test_every_element_of_packed_rows(cu, T, D, dtype):
+    check(make(1, T, D, dtype, cu=cu, seed=T + D))
+
+
+@pytest.mark.parametrize("D", [2400, 2401])
+def test_every_element_of_wide_packed_rows(D):
+    """So many columns that a block walks a packed row by itself; dlower's shares lie elsewhere."""
+    v = make(1, 600, D, "bf16", cu=[0, 100, 100, 430, 590], seed=D)
+    check(v)
+    check({**v, "dy": v["dy"][:, :, 1:2].expand(1, 600, D).contiguous(), "lower": torch.zeros_like(v["lower"])})
+
+
+def test_every_element_at_both_ends_of_all_gates():
+    for cu in (None, [0, 40, 41, 333]):
+        v = make(1, 350, 96, "fp32", cu=cu, seed=7, ends="forget")
+        check({**v, "gate": make(1, 350, 96, "fp32", seed=8, ends="gate")["gate"]})
