@@ -68,3 +68,32 @@ def test_lazily_negated_tensors_in_dropout():
     (a,) = torch.autograd.grad(dropout(leaf, 0.25, 3), leaf, dy)
     (b,) = torch.autograd.grad(dropout(leaf, 0.25, 3), leaf, dy.clone())
     assert torch.equal(a, b)
+
+
+def test_zeros_that_torch_does_not_store():
+    """Whole and sliced, as inputs and as output gradients."""
+    x, f = torch.randn(2, 9, 8, device=DEV), torch.randn(2, 9, 8, device=DEV)
+    z = torch._efficientzerotensor((4, 9, 8), device=DEV)[2:]
+    real = torch.zeros(2, 9, 8, device=DEV)
+    assert z._is_zerotensor()
+    for a, b in zip(gated_scan(x, z, z, z[0, 0], z[:, 0]), gated_scan(x, real, real, real[0, 0], real[:, 0])):
+        assert torch.equal(a, b)
+    assert torch.equal(dropout(z, 0.5, 1, residual=x), x) and torch.equal(dropout(x, 0.0, 1, residual=z), x)
+    leaf = x.clone().requires_grad_(True)
+    y, last = gated_scan(leaf, f)
+    (g,) = torch.autograd.grad((y, last), leaf, (z, z[:, 0]))
+    assert not g.any()
+    (g,) = torch.autograd.grad(dropout(leaf, 0.5, 1), leaf, z)
+    assert not g.any()
+
+
+def test_fake_outputs_do_not_reach_a_kernel():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, x1 = torch.randn(1, 9, 8, device=DEV), torch.randn(1, 8, device=DEV)
+    state = torch.zeros(1, 8, device=DEV)
+    with FakeTensorMode():
+        for call in (lambda: gated_scan(x, x), lambda: gated_scan_step(x1, x1, state), lambda: dropout(x, 0.5, 1)):
+            with pytest.raises((RuntimeError, TypeError), match="memory"):
+                call()
+    assert not state.any()

@@ -76,3 +76,47 @@ def test_a_state_that_overlaps_an_input_is_refused():
                             (wide.view(-1).as_strided((3, 2), (7, 1), 4), torch.zeros(3, 2), wide.view(-1).as_strided((3, 2), (14, 1), 9), None),
                             (pool[2:3], other[:1], pool[2:3], pool[2]), (pool[:0], other[:0], pool[:0], None)):
         refused("CUDA", x, f, st, None, lower)
+
+
+class Wrapper(torch.Tensor):
+    """A tensor that says it lies on a GPU and has no memory, at an offset."""
+
+    @staticmethod
+    def __new__(cls, *shape, dtype=torch.float32):
+        strides = torch.empty(shape, device="meta").stride()
+        return torch.Tensor._make_wrapper_subclass(cls, shape, strides=strides, dtype=dtype, device="cuda", storage_offset=64)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} was called")
+
+
+def test_tensors_without_memory_are_refused():
+    """Their data pointers are null or a small offset: no kernel may get one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        fake = torch.empty(2, 3, 4, device="cuda")[1:]
+        low, step = torch.empty(8, device="cuda")[4:], torch.empty(2, dtype=torch.int64, device="cuda")[1:]
+        cu = torch.empty(4, dtype=torch.int32, device="cuda")[1:]
+    kinds = [(fake, low, cu, step), (Wrapper(1, 3, 4), Wrapper(4), Wrapper(3, dtype=torch.int32), Wrapper(1, dtype=torch.int64))]
+    real = torch.zeros(1, 3, 4)
+    for x, low, cu, step in kinds:
+        for args in ((x, x), (real, x), (real, real, x), (real, real, None, low), (real, real, None, None, low[None] if x is fake else Wrapper(1, 4)),
+                     (real, real, None, None, None, cu)):
+            with pytest.raises(TypeError, match="memory"):
+                gated_scan(*args)
+        for args in ((x, 0.5, 1), (real, 0.5, 1, 0, x), (real, 0.5, 1, step)):
+            with pytest.raises(TypeError, match="memory"):
+                dropout(*args)
+    x2 = Wrapper(3, 4)
+    for args in ((x2, x2, x2), (real[0], real[0], x2), (real[0], real[0], real[0].clone(), x2)):
+        with pytest.raises(TypeError, match="memory"):
+            gated_scan_step(*args)
+    with pytest.raises(TypeError, match="memory"):
+        torch.vmap(lambda t: gated_scan(t, t)[0])(real[None])
+    with pytest.raises(TypeError, match="memory"):
+        gated_scan(real.to_sparse(), real)
+    zeros = torch._efficientzerotensor((3, 4))
+    with pytest.raises(ValueError, match="zeros"):
+        gated_scan_step(real[0], real[0], zeros)

@@ -48,16 +48,26 @@ int dtype_of(const Tensor& t) {
     default: return -1;
   }
 }
+// Whether t has memory behind it.  Fake tensors, wrappers of other tensors and tensors of
+// zeros that torch does not store have none, and data_ptr() of a slice of one is an offset
+// from address 0.
+bool has_memory(const Tensor& t) { return t.has_storage() && t.unsafeGetTensorImpl()->storage_initialized(); }
+// for the library: every pointer it gets comes from here
 template <typename T>
 T* ptr(const Tensor& t) {
-  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+  if (!t.defined()) return nullptr;
+  TORCH_CHECK(has_memory(t), "a tensor without memory of its own cannot go to a kernel");
+  return static_cast<T*>(t.data_ptr());
 }
-// the values as they lie in memory (a copy where torch negates them only when it reads them)
-Tensor as_stored(const Tensor& t) { return t.defined() ? t.resolve_neg() : t; }
+// the values as they lie in memory: a copy where torch negates them only when it reads
+// them, or does not store them because they are all zero
+Tensor as_stored(const Tensor& t) {
+  if (!t.defined() || !(t.is_neg() || t._is_zerotensor())) return t;
+  return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg();
+}
 // a unit stride along the last axis (a copy where it has none)
-Tensor unit_rows(const Tensor& u) {
-  const Tensor t = as_stored(u);
-  return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+Tensor unit_rows(const Tensor& t) {
+  return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? as_stored(t) : as_stored(t).contiguous();
 }
 Tensor dense(const Tensor& t) { return t.defined() ? as_stored(t).contiguous() : t; }
 // Arguments of an autograd node that may be absent.
@@ -157,24 +167,34 @@ int64_t check_states(const Tensor& x, const Tensor& state, const Tensor& cu) {
   return rows;
 }
 
-// Whether an input (rows along its first axis, or one row) shares memory with the state
-// that a step updates in place, other than element by element.
-bool clashes(const Tensor& state, const Tensor& t) {
-  if (!t.defined() || state.numel() == 0) return false;
-  const int64_t ws = state.size(-1) * state.itemsize(), wt = t.size(-1) * t.itemsize(), nt_ = t.dim() == 2 ? t.size(0) : 1,
-                ss = state.stride(0) * state.itemsize(), ts = nt_ > 1 ? t.stride(0) * t.itemsize() : 0,
-                ns = state.size(0), nt = ts == 0 ? 1 : nt_;  // a shared row is one row
-  const int64_t d = (int64_t)((intptr_t)t.data_ptr() - (intptr_t)state.data_ptr());
-  if (t.size(-1) > 1 && t.stride(-1) != 1)  // copied first
-    return false;
-  if (d >= (ns - 1) * ss + ws || d + (nt - 1) * ts + wt <= 0) return false;
+// Whether an input shares memory with the state that a step updates in place, other than
+// element by element: `ns` state rows of `ws` bytes, `ss` bytes apart, and `nt` of the
+// input's, its first byte `d` bytes behind the state's first.
+bool rows_clash(int64_t ns, int64_t ws, int64_t ss, int64_t nt, int64_t wt, int64_t ts, int64_t d) {
+  if (ts == 0) nt = 1;  // a shared row is one row
   if (d == 0 && ws == wt && ns == nt && (ns == 1 || ss == ts)) return false;
-  for (int64_t i = 0; i < ns; ++i) {  // rows that lie among one another: each row of the state
-    const int64_t at = i * ss - d, end = at - wt;  // its first byte behind t's; t's rows that end before it
+  for (int64_t i = 0; i < ns; ++i) {
+    const int64_t at = i * ss - d, end = at - wt;  // state row i from the input's first byte on; rows that end before it
     const int64_t j = ts == 0 || end < 0 ? 0 : end / ts + 1;
     if (j < nt && j * ts < at + ws && j * ts + wt > at) return true;
   }
   return false;
+}
+void check_apart(const Tensor& state, std::initializer_list<const Tensor*> inputs) {
+  const int64_t ns = state.size(0), ws = state.size(1) * 4, ss = state.stride(0) * 4;
+  if (ns == 0) return;
+  const char* const from = static_cast<const char*>(state.const_data_ptr());
+  const char* const to = from + (ns - 1) * ss + ws;
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || t->_is_zerotensor()) continue;
+    const char* const at = static_cast<const char*>(t->const_data_ptr());
+    if (at >= to) continue;
+    const int64_t e = (int64_t)t->itemsize(), wt = t->size(-1) * e, nt = t->dim() == 2 ? t->size(0) : 1,
+                  ts = nt > 1 ? t->stride(0) * e : 0;
+    if (at + (nt - 1) * ts + wt <= from || (t->size(-1) > 1 && t->stride(-1) != 1)) continue;  // apart, or copied first
+    NEED(!rows_clash(ns, ws, ss, nt, wt, ts, at - from), ValueError,
+         "gated scan: state must not share memory with other elements of an input");
+  }
 }
 
 Tensor workspace(const Inputs& in, bool backward) {
@@ -319,7 +339,10 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor tensor_of(PyObject* o, const char* what) {
   if (o == Py_None) return Tensor();
   NEED(THPVariable_Check(o), TypeError, what, " must be a tensor, got ", Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  NEED(t._is_zerotensor() || has_memory(t), TypeError, what,
+       " must be a plain tensor with memory of its own (not fake, batched, sparse or a wrapper)");
+  return t;
 }
 // a Python integer modulo 2^64
 uint64_t word_of(PyObject* o) {
@@ -361,6 +384,7 @@ PyObject* py_gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t rows = check_states(t[0], t[4], t[5]);
     check_cuda(t[0]);
     for (int i = 0; i < 3; ++i) t[i] = unit_rows(t[i]);
+    t[5] = as_stored(t[5]);
     t[3] = dense(t[3]);
     t[4] = dense(t[4]);
     Tensor y, last;
@@ -395,11 +419,11 @@ PyObject* py_gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t B = x.size(0), D = x.size(1);
     NEED((D == 1 || state.stride(1) == 1) && (B <= 1 || state.stride(0) >= D), ValueError,
          "gated scan: state rows must be contiguous and must not overlap");
-    NEED(!state.is_neg(), ValueError, "gated scan: state must not be a lazily negated view");
+    NEED(!state.is_neg() && !state._is_zerotensor(), ValueError,
+         "gated scan: state must not be a lazily negated view or a tensor of zeros without memory");
     NEED(!wants_grad({&x, &f, &g, &lower, &state}), NotImplementedError,
          "gated_scan_step has no gradients: use gated_scan, or torch.no_grad()");
-    for (const Tensor* t : {&x, &f, &g, &lower})
-      NEED(!clashes(state, *t), ValueError, "gated scan: state must not share memory with other elements of an input");
+    check_apart(state, {&x, &f, &g, &lower});
     check_cuda(x);
     x = unit_rows(x);
     f = unit_rows(f);
@@ -434,16 +458,16 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
            "dropout: residual must have x's type or be float32");
     }
     NEED(x.numel() <= (int64_t{1} << 40), ValueError, "dropout: x is too large: ", x.sizes());
-    NEED(x.is_cuda(), ValueError, "dropout: x must be on CUDA");
     Draw d{p, word_of(a[2]), 0};
     Tensor step_t;
     if (THPVariable_Check(a[3])) {
-      step_t = THPVariable_Unpack(a[3]);
+      step_t = as_stored(tensor_of(a[3], "dropout: step"));
       NEED(step_t.scalar_type() == at::kLong && step_t.numel() == 1 && step_t.device() == x.device(), ValueError,
            "dropout: a step tensor must hold one int64 on x's device");
     } else {
       d.step = word_of(a[3]);
     }
+    NEED(x.is_cuda(), ValueError, "dropout: x must be on CUDA");
     return THPVariable_Wrap(wants_grad({&x, &r})
                                 ? Dropout::apply(x, maybe(r), maybe(step_t), d.p, (int64_t)d.seed, (int64_t)d.step)
                                 : drop(x, r, d, step_t, r.defined() ? r.scalar_type() : x.scalar_type()));
