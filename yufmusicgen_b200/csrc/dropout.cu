@@ -5,10 +5,11 @@
 // residual: it draws the same words again.  One fp32 FMA, rounded once on store;
 // a dropped element is a select, so an infinite or NaN x does not get through.
 //
-// Bound by HBM: 131072 x 1024 bf16 onto an fp32 residual and its gradient 338 us for
-// 2.1 GB, 6.3 TB/s.  One pass in 16-byte pieces, 8 elements per thread; the ten rounds
-// for each 4 elements (5 wide multiplications per element) hide behind it, at 48-57 %
-// of the issue slots.
+// One pass in 16-byte pieces, 8 elements per thread.  The ten rounds for each 4 elements
+// (5 wide multiplications per element) cost the same whatever the types: 144 us for
+// 131072 x 1024 elements.  10 bytes an element hide them (bf16 onto an fp32 residual:
+// 194 us, 6.9 TB/s, bound by HBM); its gradient, 6 bytes an element, takes 145 us
+// (5.5 TB/s) and bf16 to bf16, 4 bytes, 144 us (3.7 TB/s): bound by the rounds.
 #include "gated_scan.cuh"
 #include "io_types.cuh"
 #include "philox.cuh"
@@ -33,7 +34,7 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   T v[N];
 };
 
-// `group` neighbouring elements per thread (a multiple of 4, one counter per 4)
+// G neighbouring elements per thread (a multiple of 4, one counter per 4)
 // in one row of x and res.  FLAT: x and res have no gaps, so the whole tensor
 // is one row and the index needs no division.  VEC: 16-byte accesses.
 template <typename TX, typename TO, bool RES, bool FLAT, bool VEC>

@@ -15,6 +15,8 @@ constexpr int SMS = 148;
 //   32 columns x 4096 tokens 58 / 91 against 31 / 48;  64 x 4096 58 / 91 : 53 / 80;
 //   96 x 4096 60 / 93 : 64 / 108;  128 x 4096 62 / 97 : 93 / 147;
 //   40 x 1024 21 / 34 : 19 / 30;  40 x 256 11 / 19 : 13 / 20;  10 x 256 11 / 19 : 11 / 17
+// (pairs of channels with a gate, not packed; the other types and packed rows follow the
+// same rule without having been measured on both sides).
 GatedScanPlan gated_scan_plan(int B, int T, int D, int V) {
   constexpr int L = GATED_SCAN_BLOCK;
   GatedScanPlan p;
@@ -56,8 +58,8 @@ bool gated_scan_pairs(const GatedScanArgs& a) {
 namespace {
 
 // dlower[c] = sum over rows of partial[rows, D], in 64 bits and a fixed order: 32 warps a block,
-// each every 32nd row, as many loads under way as there are rows (592 rows: 5 us with
-// 8 warps)
+// each every 32nd row, as many loads under way as there are rows (592 rows: 3.5 us;
+// 5 us with 8 warps)
 __global__ void __launch_bounds__(1024)
     gated_scan_dlower_kernel(const float* __restrict__ partial, float* __restrict__ out, long long rows, int D) {
   __shared__ double part[32][33];
@@ -76,8 +78,9 @@ __global__ void __launch_bounds__(1024)
 }
 
 // ---------------------------------------------------------------------------
-// One token per row, the state updated in place: 16 bytes of traffic per element at
-// most, bound by the launch (256x640 fp32: 4.4 us with it, 2.7 us for one row).
+// One token per row, the state updated in place: 24 bytes of traffic per element at
+// most (fp32 with a gate), bound by the launch (replayed as a graph 4.3 us for 256x640
+// fp32, whose bytes are worth 0.6, and for one row of 640 alike).
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
     gated_scan_step_kernel(const T* __restrict__ x, const T* __restrict__ f, const T* __restrict__ g, long long xs,

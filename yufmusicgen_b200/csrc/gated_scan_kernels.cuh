@@ -459,11 +459,13 @@ YUF_DEVICE void group_gates(const Raw<T, V> (&g)[N], Fv<V> (&s)[N]) {
 // ---------------------------------------------------------------------------
 // Forward, whole.  blockIdx.x = batch row * channel blocks + channel block.
 // Slots of a warp: two stages of x, f, g; y is put over x.
-// Bound by HBM where the columns fill the GPU: 16x8192x1024 bf16 with a gate 182 us,
-// 6.1 TB/s of its 1.1 GB.  With few columns by the step: 16 tokens of 16 warps load,
+// Bound by HBM where the columns fill the GPU: 16x8192x1024 bf16 with a gate 181 us,
+// 5.9 TB/s of its 1.07 GB.  With few columns by the step: 16 tokens of 16 warps load,
 // form their maps, join and run again in 3.3 us, a third of it exponentials and
-// reciprocals (two of each per element; 8x2048x640 bf16: 29 us for 84 MB).  128
-// registers hold a and i x of the run between the two passes, which allows 16 warps.
+// reciprocals (two of each per element; 8x2048x640 bf16: 29 us for 84 MB, fp32: 35 us for
+// 168 MB).  128 registers hold a and i x of the run between the two passes, which allows
+// 16 warps; without slots (plain loads) of pairs not quite, and up to 260 bytes a thread
+// are spilled.
 constexpr int fwd_slots(bool gate) { return gate ? 6 : 4; }
 
 template <typename T, int V, bool GATE, bool PACKED, bool TMA>
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     h = row_of<V>(p.h0, k.b, p.D, k.c, k.act);
   }
 
-    for (int i = 0; i < steps; ++i) {
+  for (int i = 0; i < steps; ++i) {
     const int t0 = i * stride + w * L;
     char* const sx = mine + (i & 1) * NS * SLOT;
     Raw<T, V> xr[TMA ? 1 : L], fr[TMA ? 1 : L], gr[TMA ? 1 : L];
@@ -626,7 +628,7 @@ YUF_DEVICE int range_runs(const Split& sp, int t, int T) { return max(0, min(sp.
 // The map of each range, forward: x and f; two stages.  The range is walked from its
 // end, H = sum_j (a_{j+1} ... a_last) i_j x_j, so that what the ranges kernel reads
 // first was read last here and is still in L2.  (The backward's are the other way
-// round by themselves.)  1x16384x1024 bf16: 17 us for 67 MB, started cold; half of it
+// round by themselves.)  1x16384x1024 bf16: 16 us for 67 MB, started cold; half of it
 // is the start of loads and the special function unit (55 % busy).
 template <typename T, int V, bool PACKED, bool TMA>
 __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
@@ -721,7 +723,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
 // Each range from its true start state, in one pass.  Two stages of x, f, g; y is
 // stored from registers, so that a stage is loaded again as soon as it is worked off
 // (with y staged in a third stage half as many blocks fitted: 62 us for both kernels
-// of 1x16384x1024 bf16 against 41 now).  29 us for 134 MB, started cold.
+// of 1x16384x1024 bf16, 50 without; 41 since).  27 us for 134 MB, started cold.
 template <typename T, int V, bool GATE, bool PACKED, bool TMA>
 __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     gated_scan_forward_ranges_kernel(const GatedScanArgs p, const __grid_constant__ ScanMaps tm, const Split sp) {
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
   pdl_wait();
   h = take_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), h);
 
-    for (int i = 0; i < n; ++i) {
+  for (int i = 0; i < n; ++i) {
     const int t0 = r0 + i * L;
     char* const sx = mine + (i & 1) * NS * SLOT;
     Raw<T, V> xr[TMA ? 1 : L], fr[TMA ? 1 : L], gr[TMA ? 1 : L];
@@ -849,8 +851,10 @@ __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
 // sigmoid(-f) their relative accuracy again for one reciprocal, here by the special
 // function unit alone (by turns with Newton's iteration 8x2048x640 bf16 took 77.9 us
 // forward and backward, now 76.2; the smaller of the two sigmoids kept with a sign 77.7).
-// 16x8192x1024 bf16 with a gate: 347 us, 5.5 TB/s of its 1.9 GB; bound by the latency of
-// its instructions at 16 warps per SM (h and p of the run fill the registers).
+// 16x8192x1024 bf16 with a gate: 349 us, 5.4 TB/s of its 1.9 GB; bound by the latency of
+// its instructions at 16 warps per SM (h and p of the run fill the registers).  The forms
+// without slots keep the raw rows in registers too: of pairs they spill 150 to 350 bytes a
+// thread in the whole form, 4 to 130 in ranges; of single channels up to 72.
 constexpr int bwd_slots(bool gate) { return gate ? 6 : 5; }
 
 // The block's share of dlower, the sum over its warps, to row `row` of `partial`.
@@ -945,7 +949,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
     G = take_maps<PACKED, V>(joint, at, Ranges<V>(p.work, at, (long long)p.B * sp.n_cblk), G);
   }
 
-    int seen = 0;  // steps with tokens
+  int seen = 0;  // steps with tokens
   for (int i = 0; i < steps; ++i) {
     const int t0 = t_of(i);
     char* const sx = mine + (i & 1) * 2 * SLOT;
@@ -1025,7 +1029,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
         }
       };
       if constexpr (F_ || (PACKED && (TMA || V == 1))) {
-        constexpr int N = 4;  // as many as the registers hold beside e and q
+        constexpr int N = 4;  // as many as the registers hold beside e and q (spills of 44 bytes at most)
 #pragma unroll
         for (int j0 = 0; j0 < L; j0 += N) {
           Raw<T, V> xv[N], fv[N], dv[N];
@@ -1167,7 +1171,7 @@ __global__ void __launch_bounds__(32 * NW_MAX, 1)
 }
 
 // The map of each range, backward: f, dy and g; two stages.  h is not needed.
-// 8x2048x640 bf16: 19 us for 63 MB, started cold.
+// 1x16384x1024 bf16: 24 us for 101 MB, started cold.
 template <typename T, int V, bool GATE, bool PACKED, bool TMA>
 __global__ void __launch_bounds__(32 * RANGE_WARPS, 4)
     gated_scan_backward_maps_kernel(const GatedScanArgs p, const __grid_constant__ ScanMaps tm, const Split sp) {
