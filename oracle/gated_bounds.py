@@ -12,8 +12,10 @@ u = 2^-24.  z is an argument of a sigmoid, s = sigmoid(z), m = sigmoid(-z).
   bounded in sum by M_t = a_t M_{t-1} + i_t |x_t|, M_0 = |h_0|.  Per token such a product
   takes one more rounding, the sum another, and joining runs of 16 tokens at most 3 per run:
       E_t = a_t E_{t-1} + (da_t + 4 u a_t) M_{t-1} + (em + 5 u) i_t |x_t|.
-  A run that is summed from its far end rounds its sum up to 16 times, and a state passes a
-  few joins more: 32 u M_t on top.  Second-order terms: a factor 1.05.
+  A range that is summed from its far end rounds its sum once per token without the sum
+  decaying, and a state passes a few joins more: ENDS u M_t on top, for ranges of up to 32
+  tokens (two runs: calls of up to 75776 tokens x blocks of 32 or 64 channels).  Second-order terms: a
+  factor 1.05.
 * The gradient that reaches h_t obeys the same recurrence from the end, in |dy sigmoid(g)|.
 * dlower's sum: fp32 within a run of 16 tokens, at most 24 u of its terms' magnitudes.
 Results far below the normal range flush: FLOOR.
@@ -26,6 +28,7 @@ from .gated import _sigmoid, gated_scan, gated_scan_grads, pieces
 U = 2.0**-24
 FLOOR = 1e-36
 MORE = 1.05
+ENDS = 48
 
 
 def _factors(z):
@@ -64,8 +67,8 @@ def gated_scan_bounds(x, forget, gate, lower, state, cu, dy=None, dlast=None):
             et = a[b, t] * et + (da[b, t] + 4 * U * a[b, t]) * mt + (em[b, t] + 5 * U) * ix
             mt = a[b, t] * mt + ix
             M[b, t], E[b, t] = mt, et
-        end[r] = et + 32 * U * mt if hi > lo else 0.0
-    E, Ep = MORE * (E + 32 * U * M), MORE * (Ep + 32 * U * Mp)
+        end[r] = et + ENDS * U * mt if hi > lo else 0.0
+    E, Ep = MORE * (E + ENDS * U * M), MORE * (Ep + ENDS * U * Mp)
     value = {"y": y, "last": last}
     bound = {"y": sg * (E + np.abs(h) * (esg + U)) + FLOOR, "last": MORE * end + FLOOR}
     if dy is None:
@@ -87,8 +90,8 @@ def gated_scan_bounds(x, forget, gate, lower, state, cu, dy=None, dlast=None):
             Dm[b, t], Ed[b, t] = dm, ed
             eg = a[b, t] * ed + (da[b, t] + 4 * U * a[b, t]) * dm
             gm = a[b, t] * dm
-        es0[r] = MORE * (eg + 32 * U * gm) if hi > lo else 0.0
-    Ed = MORE * (Ed + 32 * U * Dm)
+        es0[r] = MORE * (eg + ENDS * U * gm) if hi > lo else 0.0
+    Ed = MORE * (Ed + ENDS * U * Dm)
     gap = np.abs(w["prev"] - x) * live
     term = m * ((Ed + Dm * (em + 3 * U)) * gap + Dm * (Ep + U * gap)) * live
     bound["x"] = i * (Ed + Dm * (em + 4 * U)) + FLOOR
