@@ -120,3 +120,14 @@ def test_tensors_without_memory_are_refused():
     zeros = torch._efficientzerotensor((3, 4))
     with pytest.raises(ValueError, match="zeros"):
         gated_scan_step(real[0], real[0], zeros)
+
+
+def test_tangents_do_not_matter_where_forward_mode_is_off():
+    x = torch.ones(1, 3, 4)
+    with fw.dual_level():
+        dual = fw.make_dual(x, x)
+        with fw._set_fwd_grad_enabled(False):
+            for call in (lambda: gated_scan(dual, x), lambda: gated_scan_step(dual[0], x[0], x[0].clone()),
+                         lambda: dropout(dual, 0.5, 1)):
+                with pytest.raises(ValueError, match="CUDA"):  # the next refusal, on a host without a GPU
+                    call()
