@@ -8,7 +8,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
-#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -82,16 +81,13 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 // Derivatives in forward mode are not there: a tangent must not get lost in silence.  Where
-// forward mode is off (in an autograd function that carries its tangents itself) there are none.
-bool forward_mode() { return c10::AutogradState::get_tls_state().get_fw_grad_mode(); }
+// forward mode is off _fw_grad gives none.
 void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
-  if (!forward_mode()) return;
   for (const Tensor* t : ts)
     NEED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), NotImplementedError, name,
          " has no forward-mode derivatives (an input has a tangent)");
 }
 void no_tangents(const char* name, const variable_list& grads) {  // of a backward
-  if (!forward_mode()) return;
   for (const Tensor& t : grads)
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
                                 " has no forward-mode derivatives (a gradient has a tangent)");
