@@ -235,8 +235,8 @@ yuf_status_t yuf_gated_scan_backward(const void* x, const void* forget, const vo
 /* One token of B sequences: x, forget, gate (or NULL) [B, D] with row strides
  * strides [3] (NULL = contiguous), y [B, D] contiguous; state [B, D] fp32 with row
  * stride state_stride (>= D) is updated in place, e.g. a slot range of a pool.
- * The state may be x, forget or gate itself (fp32, same rows), but must not share
- * memory with other elements of an input.  B D <= 2^38. */
+ * The state may be x or forget itself (fp32, same rows), but must not share memory
+ * with the other inputs or with other elements of these.  B D <= 2^38. */
 yuf_status_t yuf_gated_scan_step(const void* x, const void* forget, const void* gate,
                                  const int64_t* strides, const float* lower, float* state,
                                  int64_t state_stride, void* y, int dtype, int B, int D,

@@ -97,3 +97,12 @@ def test_fake_outputs_do_not_reach_a_kernel():
             with pytest.raises((RuntimeError, TypeError), match="memory"):
                 call()
     assert not state.any()
+
+
+def test_a_step_may_take_its_state_as_input():
+    """Each element with itself: x and forget are the state, in rows of their own."""
+    pool = torch.randn(5, 40, device=DEV)
+    want = pool[1:4].clone()
+    y = gated_scan_step(want.clone(), want.clone(), want)
+    state = pool[1:4]
+    assert torch.equal(gated_scan_step(state, state, state), y) and torch.equal(state, want)

@@ -47,7 +47,7 @@ def test_sizes_beyond_the_limits_are_value_errors():
 
 def test_a_state_that_overlaps_an_input_is_refused():
     """The step reads its inputs while it writes the state: shared memory is allowed only
-    element by element."""
+    element by element, and not with the gate."""
     B, D = 4, 6
     pool, other = torch.zeros(B + 3, D), torch.zeros(B, D)
     wide = torch.zeros(B + 2, 3 * D + 1)
@@ -69,6 +69,9 @@ def test_a_state_that_overlaps_an_input_is_refused():
     refused("share memory", wide.view(-1).as_strided((3, 2), (7, 1), 4), torch.zeros(3, 2), wide.view(-1).as_strided((3, 2), (14, 1), 10))
     half = torch.zeros(B, D, dtype=torch.bfloat16)
     refused("share memory", other.view(torch.bfloat16)[:, :D], half, other)
+    # the gate may be read after the state has been written
+    refused("share memory", other, other, state, state)
+    refused("share memory", other, other, wide[:B, :D], wide[:B, :D])
     # nothing shared, or each element with itself: the next check answers
     for x, f, st, lower in ((state, other, state, None), (pool[:1], other[:1], pool[1:2], pool[2]), (state, state, state, pool[0]),
                             (wide[:B, :D], wide[:B, D:2 * D], wide[:B, 2 * D:3 * D], wide[B, :D]),

@@ -168,12 +168,11 @@ int64_t check_states(const Tensor& x, const Tensor& state, const Tensor& cu) {
   return rows;
 }
 
-// Whether an input shares memory with the state that a step updates in place, other than
-// element by element: `ns` state rows of `ws` bytes, `ss` bytes apart, and `nt` of the
-// input's, its first byte `d` bytes behind the state's first.
+// Whether an input shares memory with the state that a step updates in place: `ns` state
+// rows of `ws` bytes, `ss` bytes apart, and `nt` of the input's, its first byte `d` bytes
+// behind the state's first.
 bool rows_clash(int64_t ns, int64_t ws, int64_t ss, int64_t nt, int64_t wt, int64_t ts, int64_t d) {
   if (ts == 0) nt = 1;  // a shared row is one row
-  if (d == 0 && ws == wt && ns == nt && (ns == 1 || ss == ts)) return false;
   for (int64_t i = 0; i < ns; ++i) {
     const int64_t at = i * ss - d, end = at - wt;  // state row i from the input's first byte on; rows that end before it
     const int64_t j = ts == 0 || end < 0 ? 0 : end / ts + 1;
@@ -181,7 +180,7 @@ bool rows_clash(int64_t ns, int64_t ws, int64_t ss, int64_t nt, int64_t wt, int6
   }
   return false;
 }
-void check_apart(const Tensor& state, std::initializer_list<const Tensor*> inputs) {
+void check_apart(const Tensor& state, const Tensor* gate, std::initializer_list<const Tensor*> inputs) {
   const int64_t ns = state.size(0), ws = state.size(1) * 4, ss = state.stride(0) * 4;
   if (ns == 0) return;
   const char* const from = static_cast<const char*>(state.const_data_ptr());
@@ -190,11 +189,13 @@ void check_apart(const Tensor& state, std::initializer_list<const Tensor*> input
     if (!t->defined() || t->_is_zerotensor()) continue;
     const char* const at = static_cast<const char*>(t->const_data_ptr());
     if (at >= to) continue;
+    // all but the gate may be the state element by element: it is written from their values
     const int64_t e = (int64_t)t->itemsize(), wt = t->size(-1) * e, nt = t->dim() == 2 ? t->size(0) : 1,
                   ts = nt > 1 ? t->stride(0) * e : 0;
+    if (at == from && wt == ws && nt == ns && (ns == 1 || ts == ss) && t != gate) continue;
     if (at + (nt - 1) * ts + wt <= from || (t->size(-1) > 1 && t->stride(-1) != 1)) continue;  // apart, or copied first
     NEED(!rows_clash(ns, ws, ss, nt, wt, ts, at - from), ValueError,
-         "gated scan: state must not share memory with other elements of an input");
+         "gated scan: state must not share memory with an input, other than x or forget element by element");
   }
 }
 
@@ -424,7 +425,7 @@ PyObject* py_gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
          "gated scan: state must not be a lazily negated view or a tensor of zeros without memory");
     NEED(!wants_grad({&x, &f, &g, &lower, &state}), NotImplementedError,
          "gated_scan_step has no gradients: use gated_scan, or torch.no_grad()");
-    check_apart(state, {&x, &f, &g, &lower});
+    check_apart(state, &g, {&x, &f, &g, &lower});
     check_cuda(x);
     x = unit_rows(x);
     f = unit_rows(f);

@@ -46,6 +46,6 @@ def gated_scan(x, forget, gate=None, lower=None, state=None, cu_seqlens=None):
 def gated_scan_step(x, forget, state, gate=None, lower=None):
     """One token of ``B`` sequences: ``x``, ``forget``, ``gate`` ``[B, D]``; ``state
     [B, D]`` (float32, e.g. a row range of a pool of states) is updated in place; it must
-    not share memory with other elements of an input (ValueError).
+    not share memory with an input, other than x or forget element by element (ValueError).
     Returns ``y [B, D]``.  Not differentiable (NotImplementedError where that is asked for)."""
     return ops.gated_scan_step(x, forget, state, gate, lower)
